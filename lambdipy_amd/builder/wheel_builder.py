@@ -41,6 +41,10 @@ def ops_extension_path() -> Optional[str]:
     return hits[0] if hits else None
 
 
+# Device code is compiled without packed f32 instructions: some forms of
+# v_pk_{add,mul,fma}_f32 gave wrong results on MI355X (setup.py has the same).
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 HSACO_PATH = os.path.join(OPS_DIR, "standalone_gfx950.hsaco")
 HSACO_SRC = os.path.join(OPS_DIR, "csrc", "standalone.hip")
 
@@ -58,8 +62,8 @@ def ensure_standalone_hsaco(allow_build: bool = True) -> str:
         raise RuntimeError("standalone hsaco missing and allow_build=False")
     log.info("building standalone gfx950 code object (hipcc --genco)...")
     subprocess.run(
-        ["hipcc", "--genco", "--offload-arch=gfx950", "-O3", HSACO_SRC,
-         "-o", HSACO_PATH],
+        ["hipcc", "--genco", "--offload-arch=gfx950", "-O3", *NO_PACKED_F32,
+         HSACO_SRC, "-o", HSACO_PATH],
         check=True,
     )
     return HSACO_PATH
@@ -98,7 +102,7 @@ def ensure_nn_lib(allow_build: bool = True) -> str:
     objdir = os.path.join(csrc, ".nnobj")
     os.makedirs(objdir, exist_ok=True)
     flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
-             "-fvisibility=hidden", "-I", csrc]
+             "-fvisibility=hidden", "-I", csrc, *NO_PACKED_F32]
     procs = []
     objs = []
     for s in sources:

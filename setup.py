@@ -49,7 +49,10 @@ setup(
             sources=sources,
             extra_compile_args={
                 "cxx": ["-O3", "-std=c++17"],
-                "nvcc": ["-O3", "-std=c++17"],
+                # device code without packed f32 instructions: some forms of
+                # v_pk_{add,mul,fma}_f32 gave wrong results on MI355X
+                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                         "-Xclang", "-packed-fp32-ops"],
             },
         )
     ],
