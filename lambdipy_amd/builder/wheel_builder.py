@@ -69,6 +69,10 @@ def ensure_standalone_hsaco(allow_build: bool = True) -> str:
     return HSACO_PATH
 
 
+# Kernels that nn_capi.cpp has no entry for; they stay out of liblpx_nn so that
+# the torch-free layers do not grow by what they cannot call.
+TORCH_ONLY = {"rmsnorm.hip", "gemv_w4.hip", "sample.hip"}
+
 NN_LIB_PATH = os.path.join(OPS_DIR, "liblpx_nn_gfx950.so")
 
 
@@ -87,6 +91,7 @@ def ensure_nn_lib(allow_build: bool = True) -> str:
         for f in os.listdir(csrc)
         if (f.endswith(".hip") or f == "nn_capi.cpp")
         and not f.endswith("_hip.hip") and f != "standalone.hip"
+        and f not in TORCH_ONLY
     )
     headers = [os.path.join(csrc, h) for h in ("kernels.h", "lpx_common.h")]
     hdr_mtime = max(os.path.getmtime(h) for h in headers)

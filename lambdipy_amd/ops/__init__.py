@@ -30,6 +30,8 @@ from .api import (
     pairwise_sqeuclidean,
     require_extension,
     rf_predict_proba_sum,
+    rmsnorm,
+    rmsnorm_mx,
     spmv_csr,
 )
 
@@ -49,6 +51,8 @@ __all__ = [
     "matmul_mx_fp4",
     "matmul_mx_w4",
     "gemv",
+    "rmsnorm",
+    "rmsnorm_mx",
     "spmv_csr",
     "fft",
     "ifft",

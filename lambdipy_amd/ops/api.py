@@ -126,6 +126,42 @@ def matmul_mx_w4(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
     return gemm_mx_w4(qa, sa, qb, sb)
 
 
+# ---- decode-step operators on quantised weights ---------------------------
+
+def _inference_only(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} has no backward pass: call it under "
+                           "torch.no_grad() or on detached tensors")
+
+
+def rmsnorm(x: torch.Tensor, weight: torch.Tensor,
+            residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """Root-mean-square norm over the last axis, of x or of x + residual.
+
+    h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, in f32 from the
+    unrounded h, rounded once. x [..., K] bf16/fp16/f32 (rows may be strided),
+    residual like x, weight [K] of x's type or f32. Returns y, or (y, h) if a
+    residual is given: h, rounded to x's type, is the next layer's residual."""
+    _inference_only("rmsnorm", x, weight, residual)
+    out = require_extension().rmsnorm(x, weight, residual, eps)
+    return out[0] if residual is None else tuple(out)
+
+
+def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor,
+               residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """rmsnorm whose result is MX fp8, without a pass of its own for that.
+
+    x [..., K%64==0] as for rmsnorm. Returns (q, sc), or (q, sc, h) if a
+    residual is given: q [rows, K] and sc as quantize_mx gives them, ready for
+    gemm_mx, gemm_mx_w4 and gemv_mx_w4. y is quantised from f32. A block's
+    scale is the smallest power of two that brings its largest to 448 at most
+    (2^0 for a block of zeros and for the blocks that pad the last scale
+    tile); NaN and infinities become the payload's NaN."""
+    _inference_only("rmsnorm_mx", x, weight, residual)
+    return tuple(require_extension().rmsnorm_mx(x, weight, residual, eps))
+
+
 # ---- sparse --------------------------------------------------------------
 
 def spmv_csr(indptr: torch.Tensor, indices: torch.Tensor, data: torch.Tensor,

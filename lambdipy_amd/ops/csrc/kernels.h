@@ -236,6 +236,22 @@ hipError_t gemm_mx_fp4_nt8ph(const unsigned char* A, const unsigned char* sA,
                              float* C, int M, int N, int K,
                              hipStream_t stream);
 
+// ---- decode-step operators on quantised weights --------------------------
+enum class ActType { bf16, f16, f32 };
+
+// y = (x + res) * rsqrt(mean((x + res)^2) + eps) * weight, row by row; h gets
+// x + res (both ignored where res is null). x and res [R, K] with row strides
+// in elements, weight [K] of x's type or f32, h and y [R, K] contiguous.
+hipError_t rmsnorm(ActType t, const void* x, long x_stride, const void* res,
+                   long res_stride, const void* weight, bool weight_f32,
+                   float eps, void* h, void* y, int R, int K,
+                   hipStream_t stream);
+// Same with y as MX e4m3 in quantize_mx_fp8's layout (K % 64 == 0).
+hipError_t rmsnorm_mx(ActType t, const void* x, long x_stride, const void* res,
+                      long res_stride, const void* weight, bool weight_f32,
+                      float eps, void* h, unsigned char* q, unsigned char* sc,
+                      int R, int K, hipStream_t stream);
+
 // ---- torch-free serving utilities (nn_extra.hip; liblpx_nn C API) -------
 // Device randn (xorshift128 + Box-Muller), scaled: out[i] ~ N(0, scale^2).
 hipError_t randn_f32(float* out, long n, unsigned seed, float scale,

@@ -9,6 +9,8 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <cmath>
+
 #include "kernels.h"
 
 namespace {
@@ -770,6 +772,97 @@ at::Tensor conv_fp8(const at::Tensor& xq, const at::Tensor& Wq,
   return out;
 }
 
+// ---- decode-step operators on quantised weights --------------------------
+// Shapes and types are checked before the device, so that a wrong call is
+// refused for what is wrong with it on any machine.
+
+lpx::ActType act_type(const at::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return lpx::ActType::bf16;
+    case at::kHalf: return lpx::ActType::f16;
+    case at::kFloat: return lpx::ActType::f32;
+    default: TORCH_CHECK(false, what, " supports bf16, fp16 and f32, got ", t.scalar_type());
+  }
+}
+
+// Rows of a 2-D view whose last axis is dense; rows may be further apart.
+at::Tensor dense_rows(const at::Tensor& t) {
+  const at::Tensor v = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return v.size(1) == 1 || v.stride(1) == 1 ? v : v.contiguous();
+}
+
+struct NormCall {
+  at::Tensor x, w, r, h;
+  lpx::ActType type;
+  int R, K;
+};
+
+NormCall norm_call(const at::Tensor& x, const at::Tensor& weight,
+                   const std::optional<at::Tensor>& residual, double eps,
+                   const char* what) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, " expects x [..., K], K >= 1");
+  const int64_t K = x.size(-1);
+  NormCall c;
+  c.type = act_type(x, what);
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, what,
+              ": weight must be [K] = [", K, "]");
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat,
+              what, ": weight must be of x's type or f32");
+  TORCH_CHECK(std::isfinite(eps) && eps >= 0, what, ": eps must be finite and >= 0");
+  if (residual.has_value())
+    TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type(),
+                what, ": residual must have x's shape and type");
+  TORCH_CHECK(K <= (1 << 30) && x.numel() / K < (int64_t(1) << 31), what, ": too large");
+  TORCH_CHECK(x.is_cuda(), what, ": x must be on the ROCm device (got CPU)");
+  TORCH_CHECK(weight.device() == x.device() &&
+              (!residual.has_value() || residual->device() == x.device()),
+              what, ": all tensors must be on one device");
+  c.x = dense_rows(x);
+  c.w = weight.contiguous();
+  if (residual.has_value()) {
+    c.r = dense_rows(*residual);
+    c.h = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  }
+  c.R = (int)c.x.size(0);
+  c.K = (int)K;
+  return c;
+}
+
+std::vector<at::Tensor> rmsnorm(const at::Tensor& x, const at::Tensor& weight,
+                                const std::optional<at::Tensor>& residual, double eps) {
+  NormCall c = norm_call(x, weight, residual, eps, "rmsnorm");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  auto y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  check_hip(lpx::rmsnorm(c.type, c.x.data_ptr(), c.x.stride(0),
+                         c.r.defined() ? c.r.data_ptr() : nullptr,
+                         c.r.defined() ? c.r.stride(0) : 0, c.w.data_ptr(),
+                         c.w.scalar_type() == at::kFloat, (float)eps,
+                         c.r.defined() ? c.h.data_ptr() : nullptr, y.data_ptr(),
+                         c.R, c.K, current_stream(x)),
+            "rmsnorm");
+  if (c.r.defined()) return {y, c.h};
+  return {y};
+}
+
+std::vector<at::Tensor> rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight,
+                                   const std::optional<at::Tensor>& residual, double eps) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 64 == 0, "rmsnorm_mx expects x [..., K%64==0]");
+  NormCall c = norm_call(x, weight, residual, eps, "rmsnorm_mx");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  auto q = at::empty({c.R, c.K}, x.options().dtype(at::kByte));
+  auto sc = at::empty({(c.K + 127) / 128, c.R, 4}, x.options().dtype(at::kByte));
+  check_hip(lpx::rmsnorm_mx(c.type, c.x.data_ptr(), c.x.stride(0),
+                            c.r.defined() ? c.r.data_ptr() : nullptr,
+                            c.r.defined() ? c.r.stride(0) : 0, c.w.data_ptr(),
+                            c.w.scalar_type() == at::kFloat, (float)eps,
+                            c.r.defined() ? c.h.data_ptr() : nullptr,
+                            q.data_ptr<uint8_t>(), sc.data_ptr<uint8_t>(), c.R, c.K,
+                            current_stream(x)),
+            "rmsnorm_mx");
+  if (c.r.defined()) return {q, sc, c.h};
+  return {q, sc};
+}
+
 std::string build_info() {
   return std::string("lambdipy_amd ops: gfx950 (CDNA4), HIP ") +
          std::to_string(HIP_VERSION_MAJOR) + "." + std::to_string(HIP_VERSION_MINOR);
@@ -866,5 +959,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("sA"), py::arg("Bt"), py::arg("sB"));
   m.def("gemm_bf16_tune8", &gemm_bf16_tune8, "8-phase GEMM tuning variants",
         py::arg("A"), py::arg("Bt"), py::arg("tune") = 0);
+  m.def("rmsnorm", &rmsnorm, "(x + residual) normed by its root mean square",
+        py::arg("x"), py::arg("weight"), py::arg("residual") = py::none(),
+        py::arg("eps") = 1e-6);
+  m.def("rmsnorm_mx", &rmsnorm_mx, "rmsnorm -> MX e4m3 payload + E8M0 scales",
+        py::arg("x"), py::arg("weight"), py::arg("residual") = py::none(),
+        py::arg("eps") = 1e-6);
   m.def("build_info", &build_info);
 }

@@ -1,0 +1,260 @@
+// Residual addition + root-mean-square norm, with the result in the input's
+// type or as MX e4m3 (the layout that the MX GEMMs read).
+//
+//   h = x + r                        (f32; stored rounded once to x's type)
+//   y = h * (mean(h^2) + eps)^-1/2 * w
+//   MX: per 32 elements 2^e, the smallest power of two with
+//       max|y| / 2^e <= 448; payload e4m3(y / 2^e), scale byte e + 127
+//
+// The norm is taken of the unrounded f32 sum, y is rounded once, and the sum
+// of squares is held in f32 (at most 64 terms a thread, then a tree).
+//
+// One workgroup a row: the row stays in registers between the two uses of
+// it, so each input is read once and each output written once. A thread owns
+// 8 neighbouring elements a step (16-B loads of 16-bit types), an MX block is
+// four neighbouring lanes, a 128-element scale tile sixteen.
+
+#include "lpx_common.h"
+#include "kernels.h"
+
+namespace lpx {
+
+namespace {
+
+typedef __bf16 nbf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 nf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Vec8;
+template <> struct Vec8<__bf16> { typedef nbf16x8 type; };
+template <> struct Vec8<_Float16> { typedef nf16x8 type; };
+template <> struct Vec8<float> { typedef f32x8 type; };
+
+// Rows of odd length start at any multiple of the element size; global
+// memory takes wide accesses there.
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const T* p) {
+  typename Vec8<T>::type v;
+  __builtin_memcpy(&v, p, sizeof(v));
+  return __builtin_convertvector(v, f32x8);
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x8 f) {
+  const typename Vec8<T>::type v =
+      __builtin_convertvector(f, typename Vec8<T>::type);
+  __builtin_memcpy(p, &v, sizeof(v));
+}
+
+// Elements [c, c+8) of a row of K; what lies behind K is 0.
+template <typename T>
+__device__ __forceinline__ f32x8 load_row(const T* row, int c, int K) {
+  if (c + 8 <= K) return load8(row + c);
+  f32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j < K) v[j] = (float)row[c + j];
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row(T* row, int c, int K, f32x8 v) {
+  if (c + 8 <= K) {
+    store8(row + c, v);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c + j < K) row[c + j] = (T)v[j];
+}
+
+template <int TPR>
+__device__ __forceinline__ float block_sum(float v) {
+  __shared__ float part[TPR / 64];
+  v = lpx_wave_allreduce_sum(v);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < TPR / 64; ++i) v += part[i];
+  return v;
+}
+
+// E8M0 byte of a block: 448 = 1.75 * 2^8, so e = exponent - 8, one more where
+// the significand is over 1.75. A block of zeros gets 2^0.
+__device__ __forceinline__ unsigned mx_scale_byte(float amax) {
+  const unsigned b = __float_as_uint(amax);
+  if (b == 0) return 127u;
+  const int s = (int)(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u);
+  return s < 0 ? 0u : (unsigned)s;
+}
+
+// y[c .. c+8) as MX e4m3. All lanes of the wave come here together; lanes
+// with c >= K bring zeros and store nothing.
+__device__ __forceinline__ void store_mx(unsigned char* __restrict__ qrow,
+                                         unsigned char* __restrict__ sc,
+                                         int row, int R, int c, int K,
+                                         f32x8 y) {
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
+  amax = fmaxf(amax, __shfl_xor(amax, 1, 64));
+  amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
+  const unsigned byte = mx_scale_byte(amax);
+  const float scale = __uint_as_float(byte << 23);
+  unsigned tile = byte << (8 * ((threadIdx.x >> 2) & 3));
+  tile |= __shfl_xor(tile, 4, 64);
+  tile |= __shfl_xor(tile, 8, 64);
+  if (c >= K) return;
+  i32x2 out;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    s16x2 t = {0, 0};
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, y[4 * u], y[4 * u + 1],
+                                                 scale, false);
+    t = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(t, y[4 * u + 2], y[4 * u + 3],
+                                                 scale, true);
+    out[u] = __builtin_bit_cast(int, t);
+  }
+  // 64-groups are kept as their quarters [q0 | q2 | q1 | q3]
+  const int quarter = (c >> 4) & 3;
+  const int slot = ((quarter & 1) << 1) | (quarter >> 1);
+  *reinterpret_cast<i32x2*>(qrow + (c & ~63) + slot * 16 + (c & 8)) = out;
+  if ((c & 127) == 0)
+    *reinterpret_cast<unsigned*>(sc + ((long)(c >> 7) * R + row) * 4) = tile;
+}
+
+struct NormArgs {
+  const void* x;
+  const void* res;     // may be null
+  const void* weight;  // x's type, or f32
+  void* h;             // written if res is given
+  void* y;             // x's type, or the e4m3 payload
+  unsigned char* sc;
+  long x_stride, res_stride;  // elements
+  int R, K;
+  float eps;
+  bool weight_f32;
+};
+
+template <typename T, bool MX>
+__device__ __forceinline__ void finish8(const NormArgs& a, int row, int c,
+                                        f32x8 h, float inv) {
+  f32x8 w = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (c < a.K)
+    w = a.weight_f32 ? load_row((const float*)a.weight, c, a.K)
+                     : load_row((const T*)a.weight, c, a.K);
+  const f32x8 y = h * inv * w;
+  if constexpr (MX)
+    store_mx((unsigned char*)a.y + (long)row * a.K, a.sc, row, a.R, c, a.K, y);
+  else if (c < a.K)
+    store_row((T*)a.y + (long)row * a.K, c, a.K, y);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x8 read_h(const NormArgs& a, int row, int c,
+                                        bool keep) {
+  f32x8 h = load_row((const T*)a.x + (long)row * a.x_stride, c, a.K);
+  if (a.res) {
+    h += load_row((const T*)a.res + (long)row * a.res_stride, c, a.K);
+    if (keep) store_row((T*)a.h + (long)row * a.K, c, a.K, h);
+  }
+  return h;
+}
+
+__device__ __forceinline__ float square_sum(f32x8 h) {
+  float s = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s += h[j] * h[j];
+  return s;
+}
+
+// Rows of at most TPR * ITERS * 8 elements, held in registers.
+template <typename T, bool MX, int TPR, int ITERS>
+__global__ __launch_bounds__(TPR) void rmsnorm_kernel(NormArgs a) {
+  // neighbouring rows on one XCD: their scale bytes share lines of its L2
+  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
+  f32x8 h[ITERS];
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i) {
+    const int c = (i * TPR + (int)threadIdx.x) * 8;
+    h[i] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < a.K) h[i] = read_h<T>(a, row, c, true);
+    s += square_sum(h[i]);
+  }
+  const float inv = rsqrtf(block_sum<TPR>(s) / (float)a.K + a.eps);
+#pragma unroll
+  for (int i = 0; i < ITERS; ++i)
+    finish8<T, MX>(a, row, (i * TPR + (int)threadIdx.x) * 8, h[i], inv);
+}
+
+// Longer rows: read a second time (the first pass left them in the caches).
+template <typename T, bool MX>
+__global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
+  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
+  const int steps = (a.K + 8191) / 8192;
+  float s = 0.f;
+  for (int i = 0; i < steps; ++i) {
+    const int c = (i * 1024 + (int)threadIdx.x) * 8;
+    if (c < a.K) s += square_sum(read_h<T>(a, row, c, true));
+  }
+  const float inv = rsqrtf(block_sum<1024>(s) / (float)a.K + a.eps);
+  for (int i = 0; i < steps; ++i) {
+    const int c = (i * 1024 + (int)threadIdx.x) * 8;
+    f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c < a.K) h = read_h<T>(a, row, c, false);
+    finish8<T, MX>(a, row, c, h, inv);
+  }
+}
+
+template <typename T, bool MX>
+hipError_t launch(const NormArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.R);
+  if (a.K <= 2048)
+    rmsnorm_kernel<T, MX, 256, 1><<<grid, dim3(256), 0, stream>>>(a);
+  else if (a.K <= 4096)
+    rmsnorm_kernel<T, MX, 256, 2><<<grid, dim3(256), 0, stream>>>(a);
+  else if (a.K <= 8192)
+    rmsnorm_kernel<T, MX, 256, 4><<<grid, dim3(256), 0, stream>>>(a);
+  else if (a.K <= 32768)
+    rmsnorm_kernel<T, MX, 1024, 4><<<grid, dim3(1024), 0, stream>>>(a);
+  else
+    rmsnorm_long_kernel<T, MX><<<grid, dim3(1024), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <bool MX>
+hipError_t by_type(ActType t, const NormArgs& a, hipStream_t stream) {
+  if (a.R <= 0) return hipSuccess;
+  if (a.K <= 0 || (MX && a.K % 64 != 0)) return hipErrorInvalidValue;
+  switch (t) {
+    case ActType::bf16: return launch<__bf16, MX>(a, stream);
+    case ActType::f16: return launch<_Float16, MX>(a, stream);
+    case ActType::f32: return launch<float, MX>(a, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t rmsnorm(ActType t, const void* x, long x_stride, const void* res,
+                   long res_stride, const void* weight, bool weight_f32,
+                   float eps, void* h, void* y, int R, int K,
+                   hipStream_t stream) {
+  return by_type<false>(t, NormArgs{x, res, weight, h, y, nullptr, x_stride,
+                                    res_stride, R, K, eps, weight_f32},
+                        stream);
+}
+
+hipError_t rmsnorm_mx(ActType t, const void* x, long x_stride, const void* res,
+                      long res_stride, const void* weight, bool weight_f32,
+                      float eps, void* h, unsigned char* q, unsigned char* sc,
+                      int R, int K, hipStream_t stream) {
+  return by_type<true>(t, NormArgs{x, res, weight, h, q, sc, x_stride,
+                                   res_stride, R, K, eps, weight_f32},
+                       stream);
+}
+
+}  // namespace lpx

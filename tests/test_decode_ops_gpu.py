@@ -1,0 +1,268 @@
+"""The decode-step operators against plain 64-bit implementations.
+
+u(t) below is half a step of a type, the most that one rounding is off
+relative to the value: bf16 2^-8, fp16 2^-11, f32 2^-24, e4m3 2^-4.
+"""
+
+import pytest
+import torch
+
+from lambdipy_amd import ops
+
+gpu = pytest.mark.gpu
+built = pytest.mark.skipif(not ops.extension_available(),
+                           reason="extension not built")
+DEV = "cuda"
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _gen(seed):
+    return torch.Generator(device="cpu").manual_seed(seed)
+
+
+def _randn(shape, seed, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=_gen(seed)) * scale).to(dtype).to(DEV)
+
+
+# ---- residual + RMS norm ---------------------------------------------------
+
+# f32 arithmetic of a norm, relative to y: the sum of squares of n <= 2^17
+# non-negative terms is added in chains of at most 8 * 17 within a thread and
+# 22 steps across the workgroup, each off by u, the squares by 3u (two of
+# them h's): its root by half of (158 + 3)u; division, rsqrt (2 ulp) and two
+# products by at most 8u more. 90 u = 5.4e-6.
+NORM_REL = 90 * 2.0 ** -24
+
+
+def _norm64(x, weight, residual, eps):
+    h = x.double()
+    if residual is not None:
+        h = h + residual.double()
+    y = h / torch.sqrt((h * h).mean(dim=-1, keepdim=True) + eps)
+    return y * weight.double(), h
+
+
+def _near(got, want, rel, dtype):
+    """|got - want| within rel of want, or half the type's smallest step."""
+    small = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    err = (got.double() - want).abs()
+    return bool((err <= rel * want.abs() + small).all())
+
+
+NORM_SHAPES = [(1, 1), (3, 7), (1, 64), (5, 63), (2, 2048), (3, 2049),
+               (2, 4096), (1, 5003), (4, 8192), (2, 8200), (1, 32768),
+               (2, 33001), (1, 100001), (0, 128), (300, 130)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", NORM_SHAPES)
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm(rows, k, dtype, residual):
+    x = _randn((rows, k), 1, dtype, 3.0)
+    w = _randn((k,), 2, dtype)
+    r = _randn((rows, k), 3, dtype) if residual else None
+    out = ops.rmsnorm(x, w, residual=r, eps=1e-5)
+    y64, h64 = _norm64(x, w, r, 1e-5)
+    y = out[0] if residual else out
+    assert y.dtype == dtype and y.shape == x.shape
+    assert _near(y, y64, _u(dtype) + NORM_REL, dtype)
+    if residual:
+        assert out[1].dtype == dtype and out[1].shape == x.shape
+        assert _near(out[1], h64, _u(dtype) + 2.0 ** -24, dtype)
+
+
+def _mx_rows(sc, k):
+    """Tile-major scale bytes -> [rows, k/32]."""
+    return sc.permute(1, 0, 2).reshape(sc.shape[1], -1)[:, : k // 32]
+
+
+def _mx_values(q, sc):
+    rows, k = q.shape
+    d = q.view(torch.float8_e4m3fn).double().view(rows, k // 64, 4, 16)
+    d = d[:, :, [0, 2, 1, 3]].reshape(rows, k // 32, 32)
+    return (d * torch.exp2(_mx_rows(sc, k).double() - 127).unsqueeze(2)).view(rows, k)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 64), (3, 128), (7, 192), (2, 2048),
+                                    (5, 2112), (33, 4096), (2, 8192),
+                                    (3, 8256), (2, 32832), (0, 64)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_rmsnorm_mx(rows, k, dtype, residual):
+    x = _randn((rows, k), 4, dtype, 2.0)
+    # blocks whose largest elements differ by many powers of two
+    w = (_randn((k,), 5) * torch.exp2(torch.arange(k, device=DEV) // 32 % 11 - 5.0))
+    r = _randn((rows, k), 6, dtype) if residual else None
+    out = ops.rmsnorm_mx(x, w, residual=r, eps=1e-5)
+    q, sc = out[:2]
+    y64, h64 = _norm64(x, w, r, 1e-5)
+    assert q.shape == (rows, k) and q.dtype == torch.uint8
+    assert sc.shape == ((k + 127) // 128, rows, 4) and sc.dtype == torch.uint8
+    if residual:
+        assert _near(out[2], h64, _u(dtype) + 2.0 ** -24, dtype)
+    if rows == 0:
+        return
+    pad = sc.permute(1, 0, 2).reshape(rows, -1)[:, k // 32:]
+    assert bool((pad == 127).all())
+    s = torch.exp2(_mx_rows(sc, k).double() - 127)
+    amax = y64.view(rows, k // 32, 32).abs().amax(dim=2)
+    # the largest fills (224, 448] of its scale, up to y's own f32 error
+    assert bool((amax <= 448 * s * (1 + NORM_REL)).all())
+    assert bool((amax > 224 * s * (1 - NORM_REL)).all())
+    # e4m3: half a step of the value, or of its smallest numbers (2^-9)
+    step = (s * 2.0 ** -10).repeat_interleave(32, dim=1)
+    err = (_mx_values(q, sc) - y64).abs()
+    assert bool((err <= torch.maximum(2.0 ** -4 * y64.abs(), step)
+                 + 2 * NORM_REL * y64.abs()).all())
+
+
+@gpu
+def test_rmsnorm_mx_equals_quantize_of_the_plain_norm():
+    # f32 in and out: the same y goes through both quantisers
+    x = _randn((37, 1088), 7)
+    w = _randn((1088,), 8)
+    y = ops.rmsnorm(x, w)
+    q, sc = ops.rmsnorm_mx(x, w)
+    q2, sc2 = ops.quantize_mx(y)
+    assert torch.equal(q, q2)
+    assert torch.equal(_mx_rows(sc, 1088), _mx_rows(sc2, 1088))
+
+
+@gpu
+def test_rmsnorm_mx_feeds_the_mx_products():
+    # f32 in and out, so that both ways hand the same bytes to the products
+    x, w = _randn((256, 512), 9), _randn((512,), 10)
+    wq, ws = ops.quantize_mx(_randn((256, 512), 11))
+    w4, s4 = ops.quantize_mx_fp4(_randn((256, 512), 11))
+    q, sc = ops.rmsnorm_mx(x, w)
+    q2, sc2 = ops.quantize_mx(ops.rmsnorm(x, w))
+    assert torch.equal(ops.gemm_mx(q, sc, wq, ws), ops.gemm_mx(q2, sc2, wq, ws))
+    assert torch.equal(ops.gemm_mx_w4(q, sc, w4, s4),
+                       ops.gemm_mx_w4(q2, sc2, w4, s4))
+
+
+@gpu
+@pytest.mark.parametrize("mx", [False, True])
+def test_rmsnorm_strided_and_shaped(mx):
+    k = 320
+    op = ops.rmsnorm_mx if mx else ops.rmsnorm
+    wide = _randn((6, 2 * k + 3), 12, torch.bfloat16)
+    w = _randn((k,), 13, torch.bfloat16)
+    other = _randn((k, 6), 14, torch.bfloat16).t()  # columns apart
+    for x in (wide[:, :k], wide[:, 3:3 + k], wide[::2, k:2 * k],
+              wide[0, :k].expand(4, k)):
+        r = other[: x.shape[0]]
+        got = op(x, w, residual=r)
+        want = op(x.contiguous().clone(), w, residual=r.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    x3 = wide[:, :k].reshape(2, 3, k)
+    got, want = op(x3, w, residual=x3), op(wide[:, :k], w, residual=wide[:, :k])
+    assert got[-1].shape == (2, 3, k)
+    assert all(torch.equal(a.flatten(), b.flatten()) for a, b in zip(got, want))
+    one = op(wide[1, :k], w)
+    want = op(wide[1:2, :k], w)
+    a, b = (one[0], want[0]) if mx else (one, want)
+    assert torch.equal(a.flatten(), b.flatten())
+
+
+@gpu
+def test_rmsnorm_odd_values():
+    w = torch.ones(64, device=DEV)
+    # a row of zeros stays zero; its blocks have scale 1
+    z = torch.zeros(2, 64, device=DEV)
+    assert torch.equal(ops.rmsnorm(z, w), z)
+    q, sc = ops.rmsnorm_mx(z, w)
+    assert int(q.sum()) == 0 and bool((sc == 127).all())
+    # NaN and infinities reach their own row only
+    x = _randn((3, 64), 15)
+    want = ops.rmsnorm(x, w)
+    bad = x.clone()
+    bad[0, 5] = float("nan")
+    bad[2, 40] = float("inf")
+    y = ops.rmsnorm(bad, w)
+    assert bool(y[0].isnan().all()) and torch.equal(y[1], want[1])
+    assert bool(y[2, 40].isnan()) and float(y[2].nan_to_num(0).abs().sum()) == 0
+    q, sc = ops.rmsnorm_mx(bad, w)
+    v = q.view(torch.float8_e4m3fn).float()
+    assert bool(v[0].isnan().all()) and not bool(v[1].isnan().any())
+    assert int(v[2].isnan().sum()) == 1
+    # an infinite weight gives the payload's NaN, its neighbours stay finite
+    wi = w.clone()
+    wi[3] = float("inf")
+    v = ops.rmsnorm_mx(x, wi)[0].view(torch.float8_e4m3fn).float()
+    assert int(v.isnan().sum()) == 3
+    # blocks so small that the scale ends at its lowest
+    tiny = torch.full((64,), 2.0 ** -130, device=DEV)
+    q, sc = ops.rmsnorm_mx(x, tiny)
+    assert bool((sc[0, :, :2] == 0).all())
+    y64 = _norm64(x, tiny, None, 1e-6)[0]
+    err = (_mx_values(q, sc) - y64).abs()
+    assert bool((err <= torch.clamp(2.0 ** -4 * y64.abs(), min=2.0 ** -137) * 1.001).all())
+
+
+@gpu
+def test_rmsnorm_on_another_stream_and_in_a_graph():
+    x = _randn((9, 4096), 16, torch.bfloat16)
+    r = _randn((9, 4096), 17, torch.bfloat16)
+    w = _randn((4096,), 18, torch.bfloat16)
+    want = ops.rmsnorm_mx(x, w, residual=r)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.rmsnorm_mx(x, w, residual=r)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.rmsnorm_mx(x, w, residual=r)
+    for k in range(3):
+        x.copy_(_randn((9, 4096), 30 + k, torch.bfloat16))
+        g.replay()
+        want = ops.rmsnorm_mx(x, w, residual=r)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@built
+def test_rmsnorm_refuses():
+    x, w = torch.zeros(2, 64), torch.ones(64)
+    for op in (ops.rmsnorm, ops.rmsnorm_mx):
+        for bad, why in (
+                (lambda: op(x, torch.ones(65)), "weight must be"),
+                (lambda: op(x, torch.ones(1, 64)), "weight must be"),
+                (lambda: op(x, w.half()), "x's type or f32"),
+                (lambda: op(x.long(), w), "supports bf16"),
+                (lambda: op(x.double(), w), "supports bf16"),
+                (lambda: op(x, w, residual=torch.zeros(1, 64)), "residual must"),
+                (lambda: op(x, w, residual=x.half()), "residual must"),
+                (lambda: op(x, w, eps=-1.0), "eps"),
+                (lambda: op(x, w, eps=float("nan")), "eps"),
+                (lambda: op(x, w), "on the ROCm device")):
+            with pytest.raises(RuntimeError, match=why):
+                bad()
+        with pytest.raises(RuntimeError, match="no backward"):
+            op(x, w.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="K >= 1"):
+        ops.rmsnorm(torch.zeros(2, 0), torch.zeros(0))
+    with pytest.raises(RuntimeError, match="K%64"):
+        ops.rmsnorm_mx(torch.zeros(2, 65), torch.ones(65))
+
+
+# ---- 4-bit weights ---------------------------------------------------------
+
+E2M1 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0] * 2,
+                    dtype=torch.float64) * torch.tensor([1.0] * 8 + [-1.0] * 8)
+
+
+def _fp4_values(w4, sc):
+    n, k = w4.shape[0], 2 * w4.shape[1]
+    lut = E2M1.to(w4.device)
+    v = torch.stack([lut[(w4 & 15).long()], lut[(w4 >> 4).long()]], dim=2)
+    s = torch.exp2(_mx_rows(sc, k).double() - 127).unsqueeze(2)
+    return (v.view(n, k // 32, 32) * s).view(n, k)
