@@ -20,6 +20,8 @@ from .api import (
     gemm_mx_fp4,
     gemm_mx_w4,
     gemv,
+    gemv_mx_w4,
+    gemv_w4,
     ifft,
     matmul_bf16,
     matmul_mx,
@@ -51,6 +53,8 @@ __all__ = [
     "matmul_mx_fp4",
     "matmul_mx_w4",
     "gemv",
+    "gemv_w4",
+    "gemv_mx_w4",
     "rmsnorm",
     "rmsnorm_mx",
     "spmv_csr",

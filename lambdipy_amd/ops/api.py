@@ -162,6 +162,28 @@ def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor,
     return tuple(require_extension().rmsnorm_mx(x, weight, residual, eps))
 
 
+def gemv_w4(x: torch.Tensor, Bt4: torch.Tensor, sB: torch.Tensor,
+            bf16_out: bool = False) -> torch.Tensor:
+    """x @ dequant(Bt4)^T for a few rows of 16-bit activations and MX fp4
+    weights (weight-only quantisation: x is not rounded).
+
+    x [..., K] bf16 or fp16 (rows may be strided), Bt4 [N, K/2] and sB from
+    quantize_mx_fp4, any N, K%64==0. Returns [..., N] f32, or bf16. Made for
+    one to 64 rows, where reading the weights is all the time; more rows are
+    taken 64 at a time. Sums in f32, in a fixed order."""
+    _inference_only("gemv_w4", x)
+    return require_extension().gemv_w4(x, Bt4, sB, bf16_out)
+
+
+def gemv_mx_w4(A: torch.Tensor, sA: torch.Tensor, Bt4: torch.Tensor,
+               sB: torch.Tensor, bf16_out: bool = False) -> torch.Tensor:
+    """gemm_mx_w4 for a few rows: A [M, K] and sA from quantize_mx or
+    rmsnorm_mx, weights as for gemv_w4, any M and N. Both sides' values are
+    exact and their products summed in f32 (gemm_mx_w4's scaled MFMA holds
+    its inner sums less exactly)."""
+    return require_extension().gemv_mx_w4(A, sA, Bt4, sB, bf16_out)
+
+
 # ---- sparse --------------------------------------------------------------
 
 def spmv_csr(indptr: torch.Tensor, indices: torch.Tensor, data: torch.Tensor,

@@ -252,6 +252,17 @@ hipError_t rmsnorm_mx(ActType t, const void* x, long x_stride, const void* res,
                       float eps, void* h, unsigned char* q, unsigned char* sc,
                       int R, int K, hipStream_t stream);
 
+// y[M,N] (f32 or bf16) = x @ dequant(w)^T for a few rows of x (bf16 or f16,
+// row stride in elements): w fp4 [N, K/2] and scales sw in quantize_mx_fp4's
+// layout, K % 64 == 0.
+hipError_t gemv_w4(ActType t, const void* x, long x_stride,
+                   const unsigned char* w, const unsigned char* sw, void* y,
+                   bool bf16_out, int M, int N, int K, hipStream_t stream);
+// Same with x as MX e4m3 [M, K] in quantize_mx_fp8's layout.
+hipError_t gemv_mx_w4(const unsigned char* q, const unsigned char* sq,
+                      const unsigned char* w, const unsigned char* sw, void* y,
+                      bool bf16_out, int M, int N, int K, hipStream_t stream);
+
 // ---- torch-free serving utilities (nn_extra.hip; liblpx_nn C API) -------
 // Device randn (xorshift128 + Box-Muller), scaled: out[i] ~ N(0, scale^2).
 hipError_t randn_f32(float* out, long n, unsigned seed, float scale,

@@ -863,6 +863,68 @@ std::vector<at::Tensor> rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight
   return {q, sc};
 }
 
+// Weights as quantize_mx4 gives them: [N, K/2] and [ceil(K/128), N, 4].
+void check_w4(const at::Tensor& w, const at::Tensor& sw, int64_t K, const char* what) {
+  TORCH_CHECK(w.scalar_type() == at::kByte && sw.scalar_type() == at::kByte, what,
+              ": weights and scales must be byte tensors");
+  TORCH_CHECK(w.dim() == 2 && K >= 64 && K % 64 == 0 && w.size(1) * 2 == K, what,
+              ": weights must be fp4 nibbles [N, K/2], K%64==0, for activations of ", K);
+  TORCH_CHECK(sw.numel() == (K + 127) / 128 * w.size(0) * 4, what,
+              ": scale shapes must be [ceil(K/128), rows, 4] (tile-major)");
+  TORCH_CHECK(w.is_contiguous() && sw.is_contiguous(), what,
+              ": weights and scales must be contiguous");
+  TORCH_CHECK(K <= (1 << 30) && w.size(0) <= (1 << 30), what, ": too large");
+}
+
+at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor& sB,
+                   bool bf16_out) {
+  TORCH_CHECK(x.dim() >= 1, "gemv_w4 expects x [..., K]");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
+              "gemv_w4 supports bf16 and fp16 activations, got ", x.scalar_type());
+  const int64_t K = x.size(-1), N = Bt4.size(0);
+  check_w4(Bt4, sB, K, "gemv_w4");
+  TORCH_CHECK(x.numel() / K <= (1 << 19), "gemv_w4: too many rows");
+  TORCH_CHECK(x.is_cuda(), "gemv_w4: x must be on the ROCm device (got CPU)");
+  TORCH_CHECK(Bt4.device() == x.device() && sB.device() == x.device(),
+              "gemv_w4: all tensors must be on one device");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+  const at::Tensor rows = dense_rows(x);
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  auto y = at::empty(sizes, x.options()
+                                .dtype(bf16_out ? at::kBFloat16 : at::kFloat)
+                                .memory_format(at::MemoryFormat::Contiguous));
+  check_hip(lpx::gemv_w4(act_type(x, "gemv_w4"), rows.data_ptr(), rows.stride(0),
+                         Bt4.data_ptr<uint8_t>(), sB.data_ptr<uint8_t>(), y.data_ptr(),
+                         bf16_out, (int)rows.size(0), (int)N, (int)K, current_stream(x)),
+            "gemv_w4");
+  return y;
+}
+
+at::Tensor gemv_mx_w4(const at::Tensor& A, const at::Tensor& sA, const at::Tensor& Bt4,
+                      const at::Tensor& sB, bool bf16_out) {
+  TORCH_CHECK(A.scalar_type() == at::kByte && sA.scalar_type() == at::kByte,
+              "gemv_mx_w4 expects byte tensors");
+  TORCH_CHECK(A.dim() == 2, "gemv_mx_w4 expects A [M, K]");
+  const int64_t M = A.size(0), K = A.size(1), N = Bt4.size(0);
+  check_w4(Bt4, sB, K, "gemv_mx_w4");
+  TORCH_CHECK(sA.numel() == (K + 127) / 128 * M * 4,
+              "gemv_mx_w4: scale shapes must be [ceil(K/128), rows, 4] (tile-major)");
+  TORCH_CHECK(A.is_contiguous() && sA.is_contiguous(),
+              "gemv_mx_w4: activations and scales must be contiguous");
+  TORCH_CHECK(M <= (1 << 19), "gemv_mx_w4: too many rows");
+  TORCH_CHECK(A.is_cuda(), "gemv_mx_w4: A must be on the ROCm device (got CPU)");
+  TORCH_CHECK(sA.device() == A.device() && Bt4.device() == A.device() &&
+              sB.device() == A.device(), "gemv_mx_w4: all tensors must be on one device");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(A.device());
+  auto y = at::empty({M, N}, A.options().dtype(bf16_out ? at::kBFloat16 : at::kFloat));
+  check_hip(lpx::gemv_mx_w4(A.data_ptr<uint8_t>(), sA.data_ptr<uint8_t>(),
+                            Bt4.data_ptr<uint8_t>(), sB.data_ptr<uint8_t>(), y.data_ptr(),
+                            bf16_out, (int)M, (int)N, (int)K, current_stream(A)),
+            "gemv_mx_w4");
+  return y;
+}
+
 std::string build_info() {
   return std::string("lambdipy_amd ops: gfx950 (CDNA4), HIP ") +
          std::to_string(HIP_VERSION_MAJOR) + "." + std::to_string(HIP_VERSION_MINOR);
@@ -965,5 +1027,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_mx", &rmsnorm_mx, "rmsnorm -> MX e4m3 payload + E8M0 scales",
         py::arg("x"), py::arg("weight"), py::arg("residual") = py::none(),
         py::arg("eps") = 1e-6);
+  m.def("gemv_w4", &gemv_w4, "x (bf16/fp16) @ dequant(Bt4)^T, a few rows",
+        py::arg("x"), py::arg("Bt4"), py::arg("sB"), py::arg("bf16_out") = false);
+  m.def("gemv_mx_w4", &gemv_mx_w4, "x (MX e4m3) @ dequant(Bt4)^T, a few rows",
+        py::arg("A"), py::arg("sA"), py::arg("Bt4"), py::arg("sB"),
+        py::arg("bf16_out") = false);
   m.def("build_info", &build_info);
 }

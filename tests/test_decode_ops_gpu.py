@@ -78,7 +78,7 @@ def test_rmsnorm(rows, k, dtype, residual):
 
 def _mx_rows(sc, k):
     """Tile-major scale bytes -> [rows, k/32]."""
-    return sc.permute(1, 0, 2).reshape(sc.shape[1], -1)[:, : k // 32]
+    return sc.permute(1, 0, 2).flatten(1)[:, : k // 32]
 
 
 def _mx_values(q, sc):
@@ -266,3 +266,201 @@ def _fp4_values(w4, sc):
     v = torch.stack([lut[(w4 & 15).long()], lut[(w4 >> 4).long()]], dim=2)
     s = torch.exp2(_mx_rows(sc, k).double() - 127).unsqueeze(2)
     return (v.view(n, k // 32, 32) * s).view(n, k)
+
+
+def _weights(n, k, seed, lo=110, hi=140):
+    """Random nibbles and scales; the bytes that pad the last tile are NaN."""
+    w4 = torch.randint(0, 256, (n, k // 2), generator=_gen(seed), dtype=torch.uint8)
+    sc = torch.randint(lo, hi, ((k + 127) // 128, n, 4), generator=_gen(seed + 1),
+                       dtype=torch.uint8)
+    if k % 128:
+        sc[-1, :, 2:] = 255
+    return w4.to(DEV), sc.to(DEV)
+
+
+def _mx_acts(m, k, seed, lo=118, hi=136):
+    q = (_randn((m, k), seed) * 100).clamp(-448, 448).to(torch.float8_e4m3fn)
+    sc = torch.randint(lo, hi, ((k + 127) // 128, m, 4), generator=_gen(seed + 1),
+                       dtype=torch.uint8)
+    if k % 128:
+        sc[-1, :, 2:] = 255
+    return q.view(torch.uint8), sc.to(DEV)
+
+
+def _product_ok(got, x64, w64):
+    """Every product is exact in f32; k of them are summed in f32 in some
+    order: off by at most k u of the sum of their magnitudes (and fp16's
+    blocks by one more rounding each). bf16 results: half a step more."""
+    want, mag = x64 @ w64.t(), x64.abs() @ w64.abs().t()
+    tol = (x64.shape[1] + 64) * 2.0 ** -24 * mag
+    if got.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    return bool(((got.double() - want).abs() <= tol).all())
+
+
+GEMV_SHAPES = [(1, 1, 64), (1, 16, 128), (1, 17, 192), (2, 1000, 1024),
+               (5, 333, 2112), (15, 31, 320), (16, 64, 4096), (17, 100, 640),
+               (31, 257, 1088), (33, 129, 2048), (64, 64, 8192), (65, 50, 448),
+               (130, 40, 576), (0, 8, 64), (3, 0, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", GEMV_SHAPES)
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+@pytest.mark.parametrize("bf16_out", [False, True])
+def test_gemv_4bit(m, n, k, act, bf16_out):
+    w4, sw = _weights(n, k, 20)
+    if act == "mx":
+        q, sq = _mx_acts(m, k, 21)
+        got = ops.gemv_mx_w4(q, sq, w4, sw, bf16_out=bf16_out)
+        x64 = _mx_values(q, sq)
+    else:
+        x = _randn((m, k), 21, torch.bfloat16 if act == "bf16" else torch.float16, 4.0)
+        got = ops.gemv_w4(x, w4, sw, bf16_out=bf16_out)
+        x64 = x.double()
+    assert got.shape == (m, n)
+    assert got.dtype == (torch.bfloat16 if bf16_out else torch.float32)
+    if m and n:
+        assert _product_ok(got, x64, _fp4_values(w4, sw))
+
+
+@gpu
+def test_gemv_4bit_reads_what_the_quantisers_write():
+    x = _randn((7, 1088), 22, torch.bfloat16)
+    w4, sw = ops.quantize_mx_fp4(_randn((130, 1088), 23) * 0.02)
+    w64 = _fp4_values(w4, sw)
+    assert _product_ok(ops.gemv_w4(x, w4, sw), x.double(), w64)
+    q, sq = ops.quantize_mx(x.float())
+    assert _product_ok(ops.gemv_mx_w4(q, sq, w4, sw), _mx_values(q, sq), w64)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+def test_gemv_4bit_picks_out_single_weights(act):
+    # one-hot rows give back the dequantised weights, bit for bit: any mix-up
+    # of k between the two operands shows
+    k, n = 256, 48
+    w4, sw = _weights(n, k, 24)
+    for k0 in range(0, k, 64):
+        x = torch.zeros(64, k, device=DEV)
+        x[torch.arange(64), k0 + torch.arange(64)] = 1.0
+        if act == "mx":
+            got = ops.gemv_mx_w4(*ops.quantize_mx(x), w4, sw)
+        else:
+            t = torch.bfloat16 if act == "bf16" else torch.float16
+            got = ops.gemv_w4(x.to(t), w4, sw)
+        want = _fp4_values(w4, sw)[:, k0:k0 + 64].t()
+        assert torch.equal(got.double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+def test_gemv_4bit_far_scales(act):
+    # weights near the ends of f32's exponents
+    n, k = 32, 256
+    x = torch.ones(3, k, device=DEV)
+    for byte in (4, 60, 200, 240):
+        w4, sw = _weights(n, k, 25)
+        sw.fill_(byte)
+        if act == "mx":
+            got = ops.gemv_mx_w4(*ops.quantize_mx(x), w4, sw)
+        else:
+            t = torch.bfloat16 if act == "bf16" else torch.float16
+            got = ops.gemv_w4(x.to(t), w4, sw)
+        assert _product_ok(got, x.double(), _fp4_values(w4, sw))
+
+
+@gpu
+def test_gemv_4bit_nan_and_inf_stay_in_their_row():
+    w4, sw = _weights(40, 256, 26)
+    for dtype in (torch.bfloat16, torch.float16):
+        x = _randn((20, 256), 27, dtype)
+        want = ops.gemv_w4(x, w4, sw)
+        bad = x.clone()
+        bad[3, 17] = float("nan")
+        bad[18, 200] = float("inf")
+        got = ops.gemv_w4(bad, w4, sw)
+        assert bool(got[3].isnan().all())
+        assert not bool(got[18].isfinite().any())
+        keep = [i for i in range(20) if i not in (3, 18)]
+        assert torch.equal(got[keep], want[keep])
+
+
+@gpu
+def test_gemv_4bit_shapes_strides_and_repeats():
+    w4, sw = _weights(70, 320, 28)
+    wide = _randn((6, 643), 29, torch.float16)
+    for x in (wide[:, :320], wide[:, 3:323], wide[::2, 320:640],
+              wide[0, :320].expand(4, 320), _randn((320, 5), 30, torch.float16).t()):
+        got = ops.gemv_w4(x, w4, sw)
+        want = ops.gemv_w4(x.contiguous().clone(), w4, sw)
+        assert torch.equal(got, want)
+    x = wide[:, :320]
+    assert torch.equal(ops.gemv_w4(x.reshape(2, 3, 320), w4, sw).view(6, 70),
+                       ops.gemv_w4(x, w4, sw))
+    assert torch.equal(ops.gemv_w4(x[1], w4, sw), ops.gemv_w4(x[1:2], w4, sw)[0])
+    # a row's result does not depend on its neighbours
+    assert torch.equal(ops.gemv_w4(x[:1], w4, sw), ops.gemv_w4(x, w4, sw)[:1])
+    # weights that start anywhere in a buffer
+    buf = torch.zeros(w4.numel() + 5, dtype=torch.uint8, device=DEV)
+    off = buf[5:].view(w4.shape)
+    off.copy_(w4)
+    assert torch.equal(ops.gemv_w4(x, off, sw), ops.gemv_w4(x, w4, sw))
+
+
+@gpu
+def test_gemv_4bit_past_2_to_31_bytes():
+    # the last rows of 2.2 GB of weights
+    n, k = 270001, 16384
+    w4 = torch.zeros(n, k // 2, dtype=torch.uint8, device=DEV)
+    sw = torch.full((k // 128, n, 4), 127, dtype=torch.uint8, device=DEV)
+    tail, st = _weights(64, k, 31)
+    w4[-64:], sw[:, -64:] = tail, st
+    x = _randn((2, k), 32, torch.bfloat16)
+    got = ops.gemv_w4(x, w4, sw)
+    assert _product_ok(got[:, -64:], x.double(), _fp4_values(tail, st))
+    assert float(got[:, :-64].abs().max()) == 0
+
+
+@gpu
+def test_gemv_4bit_in_a_graph():
+    w4, sw = _weights(500, 1024, 33)
+    x = _randn((4, 1024), 34, torch.bfloat16)
+    ops.gemv_w4(x, w4, sw)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.gemv_w4(x, w4, sw)
+    for i in range(3):
+        x.copy_(_randn((4, 1024), 40 + i, torch.bfloat16))
+        g.replay()
+        want = ops.gemv_w4(x, w4, sw)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@built
+def test_gemv_4bit_refuses():
+    u8 = torch.uint8
+    x = torch.zeros(2, 128, dtype=torch.bfloat16)
+    w4, sw = torch.zeros(8, 64, dtype=u8), torch.zeros(1, 8, 4, dtype=u8)
+    q, sq = torch.zeros(2, 128, dtype=u8), torch.zeros(1, 2, 4, dtype=u8)
+    for bad, why in (
+            (lambda: ops.gemv_w4(x.float(), w4, sw), "bf16 and fp16"),
+            (lambda: ops.gemv_w4(x, w4.int(), sw), "byte tensors"),
+            (lambda: ops.gemv_w4(x, w4, sw.int()), "byte tensors"),
+            (lambda: ops.gemv_w4(x[:, :64], w4, sw), "fp4 nibbles"),
+            (lambda: ops.gemv_w4(x[:, :96], w4[:, :48].contiguous(), sw), "K%64"),
+            (lambda: ops.gemv_w4(x, w4.view(2, 4, 64), sw), "fp4 nibbles"),
+            (lambda: ops.gemv_w4(x, w4, sw[:, :4]), "scale shapes"),
+            (lambda: ops.gemv_w4(x, w4.t().contiguous().t(), sw), "contiguous"),
+            (lambda: ops.gemv_w4(x, w4, sw), "on the ROCm device"),
+            (lambda: ops.gemv_w4(x[:, :0], w4[:, :0], sw[:0]), "K%64"),
+            (lambda: ops.gemv_w4(torch.tensor(1.0).bfloat16(), w4, sw), "expects x"),
+            (lambda: ops.gemv_w4(x.clone().requires_grad_(), w4, sw), "no backward"),
+            (lambda: ops.gemv_mx_w4(x, sq, w4, sw), "byte tensors"),
+            (lambda: ops.gemv_mx_w4(q[0], sq, w4, sw), "expects A"),
+            (lambda: ops.gemv_mx_w4(q, sq[:, :1], w4, sw), "scale shapes"),
+            (lambda: ops.gemv_mx_w4(q.t().contiguous().t(), sq, w4, sw), "contiguous"),
+            (lambda: ops.gemv_mx_w4(q, sq, w4, sw), "on the ROCm device")):
+        with pytest.raises(RuntimeError, match=why):
+            bad()
