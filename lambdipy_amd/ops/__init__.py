@@ -34,6 +34,7 @@ from .api import (
     rf_predict_proba_sum,
     rmsnorm,
     rmsnorm_mx,
+    sample,
     spmv_csr,
 )
 
@@ -57,6 +58,7 @@ __all__ = [
     "gemv_mx_w4",
     "rmsnorm",
     "rmsnorm_mx",
+    "sample",
     "spmv_csr",
     "fft",
     "ifft",

@@ -184,6 +184,28 @@ def gemv_mx_w4(A: torch.Tensor, sA: torch.Tensor, Bt4: torch.Tensor,
     return require_extension().gemv_mx_w4(A, sA, Bt4, sB, bf16_out)
 
 
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
+           top_p=1.0, min_p=0.0) -> torch.Tensor:
+    """One token (int64) for each row of logits [..., V], bf16/fp16/f32, drawn
+    by u[row], a uniform number in [0, 1) (f32 or f64): equal inputs give
+    equal tokens. Rows may be strided, as a padded vocabulary's are.
+
+    With weights w = exp((x - max x) / temperature) and the row in falling
+    order of x, equal logits by index, what is kept is a prefix: the first
+    top_k (0: all); of these the shortest one that holds at least a share
+    top_p of their weight (1: all, and always the first); and of it what has
+    w >= min_p. The token is the first in that order whose running weight
+    exceeds u times the kept weight. temperature 0 takes the largest logit,
+    the first of equal ones. Each setting is a number or a tensor with one
+    value for each row on the logits' device (top_k int32 or int64, the others
+    f32 or f64); a tensor's values are not looked at on the host: a
+    temperature that is not positive counts as 0, top_k below 1 as 0.
+
+    NaN logits count as -inf. +inf logits share a row equally. A row in which
+    nothing is over -inf gives -1."""
+    return require_extension().sample(logits, u, temperature, top_k, top_p, min_p)
+
+
 # ---- sparse --------------------------------------------------------------
 
 def spmv_csr(indptr: torch.Tensor, indices: torch.Tensor, data: torch.Tensor,

@@ -263,6 +263,22 @@ hipError_t gemv_mx_w4(const unsigned char* q, const unsigned char* sq,
                       const unsigned char* w, const unsigned char* sw, void* y,
                       bool bf16_out, int M, int N, int K, hipStream_t stream);
 
+// A setting of each row: one value for all, or an array of one per row.
+struct SampleParam {
+  enum Kind { value_, f32, f64, i32, i64 };
+  const void* ptr;
+  double value;
+  Kind kind;
+};
+// token[r]: drawn from row r of logits [rows, vocab] (row stride in elements)
+// by u[r] after temperature, top-k, top-p and min-p; -1 where a row has no
+// logit over -inf. workspace: sample_workspace(rows, vocab) bytes.
+size_t sample_workspace(int rows, int vocab);
+hipError_t sample(ActType t, const void* logits, long stride, int rows,
+                  int vocab, SampleParam temperature, SampleParam top_k,
+                  SampleParam top_p, SampleParam min_p, SampleParam u,
+                  void* workspace, int64_t* token, hipStream_t stream);
+
 // ---- torch-free serving utilities (nn_extra.hip; liblpx_nn C API) -------
 // Device randn (xorshift128 + Box-Muller), scaled: out[i] ~ N(0, scale^2).
 hipError_t randn_f32(float* out, long n, unsigned seed, float scale,

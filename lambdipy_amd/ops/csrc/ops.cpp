@@ -10,6 +10,8 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
 #include <cmath>
+#include <limits>
+#include <variant>
 
 #include "kernels.h"
 
@@ -925,6 +927,62 @@ at::Tensor gemv_mx_w4(const at::Tensor& A, const at::Tensor& sA, const at::Tenso
   return y;
 }
 
+// A setting of `sample`: a number, or one for each row.
+using Setting = std::variant<at::Tensor, double>;
+
+lpx::SampleParam setting(const Setting& v, const char* name, int64_t rows, bool whole,
+                         double least, double most, const at::Tensor& logits,
+                         std::vector<at::Tensor>& keep) {
+  if (std::holds_alternative<double>(v)) {
+    const double d = std::get<double>(v);
+    TORCH_CHECK(d >= least && d <= most, "sample: ", name, " must be in [", least, ", ",
+                most, "], got ", d);
+    return {nullptr, d, lpx::SampleParam::value_};
+  }
+  const at::Tensor& t = std::get<at::Tensor>(v);
+  const auto type = t.scalar_type();
+  TORCH_CHECK(t.dim() <= 1 || t.sizes() == logits.sizes().slice(0, logits.dim() - 1),
+              "sample: ", name, " must have one value for each row");
+  TORCH_CHECK(t.numel() == rows, "sample: ", name, " must have one value for each row");
+  TORCH_CHECK(whole ? type == at::kInt || type == at::kLong
+                    : type == at::kFloat || type == at::kDouble,
+              "sample: ", name, " must be ", whole ? "int32 or int64" : "f32 or f64");
+  TORCH_CHECK(t.device() == logits.device(), "sample: ", name,
+              " must be on the logits' device");
+  keep.push_back(t.contiguous());
+  return {keep.back().data_ptr(), 0.0,
+          type == at::kInt    ? lpx::SampleParam::i32
+          : type == at::kLong ? lpx::SampleParam::i64
+          : type == at::kFloat ? lpx::SampleParam::f32
+                               : lpx::SampleParam::f64};
+}
+
+at::Tensor sample(const at::Tensor& logits, const at::Tensor& u, const Setting& temperature,
+                  const Setting& top_k, const Setting& top_p, const Setting& min_p) {
+  TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "sample expects logits [..., V], V >= 1");
+  const auto type = act_type(logits, "sample");
+  const int64_t V = logits.size(-1), rows = logits.numel() / V;
+  TORCH_CHECK(V <= (1 << 24) && rows < (int64_t(1) << 31), "sample: too large");
+  std::vector<at::Tensor> keep;
+  const double top = std::numeric_limits<double>::max();
+  const auto t = setting(temperature, "temperature", rows, false, 0, top, logits, keep);
+  const auto k = setting(top_k, "top_k", rows, true, 0, top, logits, keep);
+  const auto p = setting(top_p, "top_p", rows, false, 0, 1, logits, keep);
+  const auto q = setting(min_p, "min_p", rows, false, 0, 1, logits, keep);
+  const auto draw = setting(u, "u", rows, false, 0, 1, logits, keep);
+  TORCH_CHECK(logits.is_cuda(), "sample: logits must be on the ROCm device (got CPU)");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  const at::Tensor x = dense_rows(logits);
+  auto token = at::empty(logits.sizes().slice(0, logits.dim() - 1),
+                         logits.options().dtype(at::kLong));
+  auto work = at::empty({(int64_t)lpx::sample_workspace((int)rows, (int)V)},
+                        logits.options().dtype(at::kByte));
+  check_hip(lpx::sample(type, x.data_ptr(), x.stride(0), (int)rows, (int)V, t, k, p, q, draw,
+                        work.data_ptr(), token.data_ptr<int64_t>(), current_stream(logits)),
+            "sample");
+  return token;
+}
+
 std::string build_info() {
   return std::string("lambdipy_amd ops: gfx950 (CDNA4), HIP ") +
          std::to_string(HIP_VERSION_MAJOR) + "." + std::to_string(HIP_VERSION_MINOR);
@@ -1032,5 +1090,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemv_mx_w4", &gemv_mx_w4, "x (MX e4m3) @ dequant(Bt4)^T, a few rows",
         py::arg("A"), py::arg("sA"), py::arg("Bt4"), py::arg("sB"),
         py::arg("bf16_out") = false);
+  m.def("sample", &sample, "one token for each row of logits",
+        py::arg("logits"), py::arg("u"), py::arg("temperature") = 1.0,
+        py::arg("top_k") = 0.0, py::arg("top_p") = 1.0, py::arg("min_p") = 0.0);
   m.def("build_info", &build_info);
 }

@@ -1,0 +1,570 @@
+// One token for each row of logits: temperature, top-k, top-p, min-p and the
+// draw, from a given uniform number.
+//
+//   w_i = exp((x_i - max x) / T), the row in the order (x falling, i rising);
+//   kept is a prefix of that order: the shortest of the first k, of the
+//   shortest one holding a share p of those k's weight, and of w_i >= min_p;
+//   the token is the first whose running weight exceeds u times the kept.
+//
+// All three filters and the draw ask the same thing of the sorted row: where
+// does a running count or a running weight pass a border. Nothing is sorted
+// for that. Weights are 64-bit integers (w_i * 2^45, rounded), so their sums
+// do not depend on the order of adding and a histogram's totals agree with
+// its members' to the last bit: 256 bins, linear in x below the maximum, tell
+// the bin that holds a border, and only that bin's members are looked at.
+//
+// Three launches: the maxima of chunks of rows; the chunks' histograms (one
+// exp a logit, in 64 bits: a border in a flat row of 10^5 logits is decided by
+// the 10th digit of a sum); one workgroup a row that finds the borders.
+
+#include "lpx_common.h"
+#include "kernels.h"
+
+namespace lpx {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr int BINS = 256;
+constexpr int CHUNK_THREADS = 256;
+constexpr int ROW_THREADS = 1024;
+constexpr int LIST = 4096;  // members of bins kept in LDS
+constexpr int FEW = 64;     // members that one wave ranks
+
+struct ChunkMax {
+  float hi, lo;  // largest; smallest that is not -inf
+  int at;        // lowest index of the largest
+};
+
+struct ChunkBins {
+  u64 mass[BINS];
+  unsigned count[BINS];
+  u64 minp;  // mass of w >= min_p
+};
+
+struct SampleArgs {
+  const void* logits;
+  long stride;  // elements
+  int rows, vocab, chunk, chunks, shift;
+  SampleParam temperature, top_k, top_p, min_p, u;
+  ChunkMax* maxima;  // [rows][chunks]
+  ChunkBins* bins;   // [rows][chunks]
+  int64_t* token;
+};
+
+__device__ __forceinline__ double param(const SampleParam& p, int row) {
+  switch (p.kind) {
+    case SampleParam::f32: return static_cast<const float*>(p.ptr)[row];
+    case SampleParam::f64: return static_cast<const double*>(p.ptr)[row];
+    case SampleParam::i32: return static_cast<const int*>(p.ptr)[row];
+    case SampleParam::i64: return (double)static_cast<const int64_t*>(p.ptr)[row];
+    default: return p.value;
+  }
+}
+
+__device__ __forceinline__ float as_f32(float x) { return x; }
+__device__ __forceinline__ float as_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float as_f32(__bf16 x) { return (float)x; }
+
+// f(index, logit) for every logit of [begin, end) that a token can be drawn
+// from: not NaN, not -inf. A thread's indices rise.
+// AHEAD: 16-B loads in flight a thread.
+template <int THREADS, int AHEAD, typename T, typename F>
+__device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
+                                     int end, F f) {
+  constexpr int VEC = 16 / sizeof(T);
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  auto one = [&](int i, float x) {
+    if (x > -__builtin_inff()) f(i, x + 0.f);  // -0 is 0
+  };
+  const int tid = (int)threadIdx.x;
+  const int off = (int)(((uintptr_t)(row + begin) & 15) / sizeof(T));
+  const int head = min(off ? VEC - off : 0, end - begin);
+  if (tid < head) one(begin + tid, as_f32(row[begin + tid]));
+  const int first = begin + head;
+  const int vecs = (end - first) / VEC;
+  const V* body = reinterpret_cast<const V*>(row + first);
+  for (int i = tid; i < vecs; i += AHEAD * THREADS) {
+    V v[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (i + a * THREADS < vecs) v[a] = body[i + a * THREADS];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (i + a * THREADS >= vecs) break;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        one(first + (i + a * THREADS) * VEC + j, as_f32(v[a][j]));
+    }
+  }
+  const int tail = first + vecs * VEC + tid;
+  if (tail < end) one(tail, as_f32(row[tail]));
+}
+
+// ---- a row's weights and bins --------------------------------------------
+
+struct RowScale {
+  float hi;       // the row's largest logit
+  double inv_t;
+  double one;     // 2^shift
+  float per_bin;  // bins per unit of x
+  int at;
+  bool greedy;
+};
+
+// The largest logit with its lowest index, and the smallest.
+struct Extent {
+  float hi = -__builtin_inff(), lo = __builtin_inff();
+  int at = 0x7fffffff;
+  __device__ __forceinline__ void join(float h, float l, int i) {
+    if (h > hi || (h == hi && i < at)) {
+      hi = h;
+      at = i;
+    }
+    lo = fminf(lo, l);
+  }
+  __device__ __forceinline__ void join_wave() {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1)
+      join(__shfl_xor(hi, m, 64), __shfl_xor(lo, m, 64), __shfl_xor(at, m, 64));
+  }
+};
+
+// Every wave works it out for itself: the same bits in every kernel.
+__device__ __forceinline__ RowScale row_scale(const SampleArgs& a, int row) {
+#pragma clang fp contract(off)
+  const ChunkMax* c = a.maxima + (long)row * a.chunks;
+  Extent e;
+  for (int i = (int)threadIdx.x & 63; i < a.chunks; i += 64)
+    e.join(c[i].hi, c[i].lo, c[i].at);
+  e.join_wave();
+  const float lo = e.lo;
+  RowScale r;
+  r.hi = e.hi;
+  r.at = e.hi > -__builtin_inff() ? e.at : -1;
+  const double t = param(a.temperature, row);
+  r.greedy = !(t > 0) || r.at < 0;
+  r.inv_t = 1.0 / t;
+  r.one = __builtin_ldexp(1.0, a.shift);
+  // Below 32 T the weight rounds to nothing (e^-32 < 2^-46).
+  const double reach = fmin((double)r.hi - (double)lo, 32.0 * t);
+  const double per = BINS / reach;
+  r.per_bin = reach > 0 && per < 1e30 ? (float)per : reach > 0 ? 1e30f : 0.f;
+  return r;
+}
+
+__device__ __forceinline__ int bin_of(const RowScale& r, float x) {
+#pragma clang fp contract(off)
+  // monotone in x; infinities and 0 * inf end in the last bin
+  const float d = x == r.hi ? 0.f : r.hi - x;
+  return (int)fminf(d * r.per_bin, (float)(BINS - 1));
+}
+
+// The same bits wherever it is inlined: nothing here may be contracted in
+// one place and not in another.
+__device__ __forceinline__ u64 weight(const RowScale& r, float x) {
+#pragma clang fp contract(off)
+  if (x == r.hi) return (u64)r.one;
+  const double t = ((double)x - (double)r.hi) * r.inv_t;
+  const double w = exp(t) * r.one;
+  return w > 0 ? (u64)(w + 0.5) : 0;
+}
+
+// ---- 1: maxima ------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(CHUNK_THREADS) void chunk_max_kernel(SampleArgs a) {
+  const int row = (int)blockIdx.x / a.chunks;
+  const int begin = (int)blockIdx.x % a.chunks * a.chunk;
+  const int end = min(begin + a.chunk, a.vocab);
+  Extent e;
+  scan<CHUNK_THREADS, 2>(static_cast<const T*>(a.logits) + row * a.stride, begin,
+                         end, [&](int i, float x) { e.join(x, x, i); });
+  e.join_wave();
+  __shared__ ChunkMax part[CHUNK_THREADS / 64];
+  if ((threadIdx.x & 63) == 0)
+    part[threadIdx.x >> 6] = ChunkMax{e.hi, e.lo, e.at};
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int i = 1; i < CHUNK_THREADS / 64; ++i)
+    e.join(part[i].hi, part[i].lo, part[i].at);
+  a.maxima[blockIdx.x] = ChunkMax{e.hi, e.lo, e.at};
+}
+
+// ---- 2: histograms --------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a) {
+  const int row = (int)blockIdx.x / a.chunks;
+  const int begin = (int)blockIdx.x % a.chunks * a.chunk;
+  const int end = min(begin + a.chunk, a.vocab);
+  const RowScale r = row_scale(a, row);
+  if (r.greedy) return;
+  __shared__ ChunkBins b;
+  b.mass[threadIdx.x] = 0;
+  b.count[threadIdx.x] = 0;
+  if (threadIdx.x == 0) b.minp = 0;
+  __syncthreads();
+  const double least = param(a.min_p, row) * r.one;
+  u64 minp = 0;
+  scan<CHUNK_THREADS, 2>(static_cast<const T*>(a.logits) + row * a.stride, begin,
+                      end, [&](int, float x) {
+                        const int bin = bin_of(r, x);
+                        const u64 w = weight(r, x);
+                        atomicAdd(&b.count[bin], 1u);
+                        if (w) atomicAdd(&b.mass[bin], w);
+                        if ((double)w >= least) minp += w;
+                      });
+  atomicAdd(&b.minp, minp);
+  __syncthreads();
+  ChunkBins& out = a.bins[blockIdx.x];
+  out.mass[threadIdx.x] = b.mass[threadIdx.x];
+  out.count[threadIdx.x] = b.count[threadIdx.x];
+  if (threadIdx.x == 0) out.minp = b.minp;
+}
+
+// ---- 3: borders -----------------------------------------------------------
+
+// Sorts ascending as (x falling, index rising); no two are equal.
+__device__ __forceinline__ u64 order_of(float x, int i) {
+  const unsigned b = __float_as_uint(x);
+  const unsigned up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  return ((u64)~up << 32) | (unsigned)i;
+}
+
+__device__ __forceinline__ float logit_of(u64 o) {
+  const unsigned up = ~(unsigned)(o >> 32);
+  return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
+}
+
+struct Bins {
+  u64 mass[BINS];
+  unsigned count[BINS];
+};
+
+struct RowShared {
+  Bins row, sub;  // running sums, bin by bin
+  u64 list[LIST];
+  u64 few[FEW];
+  u64 wave_mass[BINS / 64];
+  unsigned wave_count[BINS / 64];
+  u64 lo, hi;
+  u64 minp;
+  unsigned n;
+  int bin;
+  u64 mass;  // a border's answer
+  int at;
+};
+
+// Counts and masses of bins -> running sums.
+__device__ __forceinline__ void run_up(Bins& b, RowShared& sh) {
+  const int t = (int)threadIdx.x, lane = t & 63;
+  u64 m = 0;
+  unsigned c = 0;
+  if (t < BINS) {
+    m = b.mass[t];
+    c = b.count[t];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const u64 mm = __shfl_up(m, d, 64);
+      const unsigned cc = __shfl_up(c, d, 64);
+      if (lane >= d) {
+        m += mm;
+        c += cc;
+      }
+    }
+    if (lane == 63) {
+      sh.wave_mass[t >> 6] = m;
+      sh.wave_count[t >> 6] = c;
+    }
+  }
+  __syncthreads();
+  if (t < BINS) {
+    for (int w = 0; w < (t >> 6); ++w) {
+      m += sh.wave_mass[w];
+      c += sh.wave_count[w];
+    }
+    b.mass[t] = m;
+    b.count[t] = c;
+  }
+  __syncthreads();
+}
+
+// The first bin whose running sum reaches `border`, which some bin's does.
+__device__ __forceinline__ int bin_at(const Bins& b, bool by_count, u64 border,
+                                      RowShared& sh) {
+  const int t = (int)threadIdx.x;
+  if (t == 0) sh.bin = BINS - 1;
+  __syncthreads();
+  if (t < BINS) {
+    const u64 now = by_count ? b.count[t] : b.mass[t];
+    const u64 before = t == 0 ? 0 : by_count ? b.count[t - 1] : b.mass[t - 1];
+    if (now >= border && before < border) sh.bin = t;
+  }
+  __syncthreads();
+  const int bin = sh.bin;
+  __syncthreads();
+  return bin;
+}
+
+template <typename T>
+struct RowPick {
+  const SampleArgs& a;
+  const T* row;
+  const RowScale r;
+  RowShared& sh;
+  int first = 0, last = -1;  // the bins whose members are in the list
+
+  // f(order, logit) of the members of `bin` between lo and hi
+  template <typename F>
+  __device__ __forceinline__ void members(int bin, u64 lo, u64 hi, F f) {
+    if (first <= bin && bin <= last) {
+      const int n = (int)min(sh.n, (unsigned)LIST);
+      for (int i = (int)threadIdx.x; i < n; i += ROW_THREADS) {
+        const u64 o = sh.list[i];
+        const float x = logit_of(o);
+        if (bin_of(r, x) == bin && lo <= o && o <= hi) f(o, x);
+      }
+    } else {
+      scan<ROW_THREADS, 1>(row, 0, a.vocab, [&](int i, float x) {
+        if (bin_of(r, x) != bin) return;
+        const u64 o = order_of(x, i);
+        if (lo <= o && o <= hi) f(o, x);
+      });
+    }
+  }
+
+  __device__ __forceinline__ unsigned through(int bin) const {
+    return bin < 0 ? 0 : sh.row.count[bin];
+  }
+
+  // Lists the members of bins [from, to], of which there are at most LIST.
+  __device__ __forceinline__ void collect(int from, int to) {
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    scan<ROW_THREADS, 4>(row, 0, a.vocab, [&](int i, float x) {
+      const int bin = bin_of(r, x);
+      if (from <= bin && bin <= to) {
+        const unsigned n = atomicAdd(&sh.n, 1u);
+        if (n < LIST) sh.list[n] = order_of(x, i);
+      }
+    });
+    __syncthreads();
+    first = from;
+    last = to;
+  }
+
+  // The member of the row at which the running count (mass) reaches `border`:
+  // its index to sh.at, the running mass with it to sh.mass.
+  __device__ __forceinline__ void resolve(bool by_count, u64 border) {
+    const int bin = bin_at(sh.row, by_count, border, sh);
+    unsigned base = through(bin - 1), n = sh.row.count[bin] - base;
+    u64 mass = bin ? sh.row.mass[bin - 1] : 0;
+    if (!(first <= bin && bin <= last) && n <= LIST) collect(bin, bin);
+    u64 lo = 0, hi = ~0ull;
+    while (n > FEW) {
+      // 256 sub-bins between the first and the last member; the two differ,
+      // so that n falls with every turn
+      if (threadIdx.x == 0) {
+        sh.lo = ~0ull;
+        sh.hi = 0;
+      }
+      if (threadIdx.x < BINS) {
+        sh.sub.mass[threadIdx.x] = 0;
+        sh.sub.count[threadIdx.x] = 0;
+      }
+      __syncthreads();
+      u64 tlo = ~0ull, thi = 0;
+      members(bin, lo, hi, [&](u64 o, float) {
+        tlo = min(tlo, o);
+        thi = max(thi, o);
+      });
+      if (tlo <= thi) {
+        atomicMin(&sh.lo, tlo);
+        atomicMax(&sh.hi, thi);
+      }
+      __syncthreads();
+      lo = sh.lo;
+      hi = sh.hi;
+      const int drop = max(0, 64 - __clzll((long long)(hi - lo)) - 8);
+      members(bin, lo, hi, [&](u64 o, float x) {
+        const int s = (int)((o - lo) >> drop);
+        atomicAdd(&sh.sub.count[s], 1u);
+        const u64 w = weight(r, x);
+        if (w) atomicAdd(&sh.sub.mass[s], w);
+      });
+      __syncthreads();
+      run_up(sh.sub, sh);
+      const int s = bin_at(sh.sub, by_count, border - (by_count ? base : mass), sh);
+      const unsigned before = s ? sh.sub.count[s - 1] : 0;
+      n = sh.sub.count[s] - before;
+      base += before;
+      mass += s ? sh.sub.mass[s - 1] : 0;
+      lo += (u64)s << drop;
+      hi = lo + min(hi - lo, (1ull << drop) - 1);
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+      sh.bin = 0;
+      sh.at = r.at;
+      sh.mass = mass;
+    }
+    __syncthreads();
+    members(bin, lo, hi, [&](u64 o, float) {
+      const int i = atomicAdd(&sh.bin, 1);
+      if (i < FEW) sh.few[i] = o;
+    });
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const bool mine = threadIdx.x < n;
+      const u64 o = mine ? sh.few[threadIdx.x] : ~0ull;
+      const u64 w = mine ? weight(r, logit_of(o)) : 0;
+      unsigned before = 0;
+      u64 run = 0;
+      for (unsigned j = 0; j < n; ++j) {
+        const u64 oj = __shfl(o, j, 64), wj = __shfl(w, j, 64);
+        if (oj < o) {
+          ++before;
+          run += wj;
+        }
+      }
+      const u64 now = by_count ? base + before + 1 : mass + run + w;
+      const u64 was = by_count ? base + before : mass + run;
+      if (mine && now >= border && was < border) {
+        sh.mass = mass + run + w;
+        sh.at = (int)(unsigned)o;
+      }
+    }
+    __syncthreads();
+  }
+};
+
+template <typename T>
+__global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
+  __shared__ RowShared sh;
+  const int row = (int)blockIdx.x, t = (int)threadIdx.x;
+  const RowScale r = row_scale(a, row);
+  if (r.greedy) {
+    if (t == 0) a.token[row] = r.at;
+    return;
+  }
+  if (t < BINS) {
+    sh.row.mass[t] = 0;
+    sh.row.count[t] = 0;
+  }
+  if (t == 0) sh.minp = 0;
+  __syncthreads();
+  {
+    const ChunkBins* c = a.bins + (long)row * a.chunks;
+    u64 m = 0;
+    unsigned n = 0;
+    const int bin = t % BINS;
+    for (int i = t / BINS; i < a.chunks; i += ROW_THREADS / BINS) {
+      m += c[i].mass[bin];
+      n += c[i].count[bin];
+    }
+    atomicAdd(&sh.row.mass[bin], m);
+    atomicAdd(&sh.row.count[bin], n);
+    if (t < a.chunks) atomicAdd(&sh.minp, c[t].minp);
+    for (int i = t + ROW_THREADS; i < a.chunks; i += ROW_THREADS)
+      atomicAdd(&sh.minp, c[i].minp);
+  }
+  __syncthreads();
+  run_up(sh.row, sh);
+
+  const u64 total = sh.row.mass[BINS - 1];
+  const unsigned all = sh.row.count[BINS - 1];
+  const double k = param(a.top_k, row), p = param(a.top_p, row);
+  RowPick<T> pick{a, static_cast<const T*>(a.logits) + row * a.stride, r, sh};
+
+  // what a share of a mass has to reach
+  auto share = [](double part, u64 of) {
+    const double s = ceil(part * (double)of);
+    return s >= (double)of ? of : s > 1 ? (u64)s : (u64)1;
+  };
+  u64 kept = total;
+  const bool by_k = k >= 1 && k < (double)all, by_p = p < 1;
+  if (by_k) {
+    const unsigned want = (unsigned)k;
+    const int bin = bin_at(sh.row, true, want, sh);
+    if (sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    if (sh.row.count[bin] == want) {
+      kept = sh.row.mass[bin];
+    } else {
+      pick.resolve(true, want);
+      kept = sh.mass;
+    }
+  }
+  if (by_p) {
+    const u64 border = share(p, kept);
+    const int bin = bin_at(sh.row, false, border, sh);
+    if (pick.last < bin && sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    pick.resolve(false, border);
+    kept = sh.mass;
+  }
+  kept = min(kept, sh.minp);
+  const double at = floor(param(a.u, row) * (double)kept);
+  const u64 border = 1 + (at > 0 ? (at >= (double)kept ? kept - 1 : min((u64)at, kept - 1)) : 0);
+  pick.resolve(false, border);
+  if (t == 0) a.token[row] = sh.at;
+}
+
+template <typename T>
+hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
+  chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+  chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+  row_pick_kernel<T>
+      <<<dim3((unsigned)a.rows), dim3(ROW_THREADS), 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+struct Plan {
+  int chunk, chunks;
+  size_t maxima_bytes, bytes;
+};
+
+Plan plan_of(int rows, int vocab) {
+  // At least 4096 logits a chunk; more where there are chunks enough for the
+  // chip without that, so that fewer histograms are written.
+  const long want = ((long)rows * vocab + 2047) / 2048;
+  Plan p;
+  p.chunk = (int)(want < 4096 ? 4096 : (want + 511) / 512 * 512);
+  p.chunks = (vocab + p.chunk - 1) / p.chunk;
+  p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
+  p.bytes = p.maxima_bytes + (size_t)rows * p.chunks * sizeof(ChunkBins);
+  return p;
+}
+
+}  // namespace
+
+size_t sample_workspace(int rows, int vocab) {
+  return rows > 0 && vocab > 0 ? plan_of(rows, vocab).bytes : 0;
+}
+
+hipError_t sample(ActType t, const void* logits, long stride, int rows,
+                  int vocab, SampleParam temperature, SampleParam top_k,
+                  SampleParam top_p, SampleParam min_p, SampleParam u,
+                  void* workspace, int64_t* token, hipStream_t stream) {
+  if (rows <= 0) return hipSuccess;
+  if (vocab <= 0) return hipErrorInvalidValue;
+  const Plan p = plan_of(rows, vocab);
+  if ((int64_t)rows * p.chunks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
+  int shift = 45;  // sums of `vocab` weights stay below 2^62
+  while (vocab > (int64_t(1) << (62 - shift))) --shift;
+  SampleArgs a{logits, stride, rows, vocab, p.chunk, p.chunks, shift,
+               temperature, top_k, top_p, min_p, u,
+               static_cast<ChunkMax*>(workspace),
+               reinterpret_cast<ChunkBins*>(static_cast<char*>(workspace) +
+                                            p.maxima_bytes),
+               token};
+  switch (t) {
+    case ActType::bf16: return launch<__bf16>(a, stream);
+    case ActType::f16: return launch<_Float16>(a, stream);
+    case ActType::f32: return launch<float>(a, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace lpx

@@ -464,3 +464,238 @@ def test_gemv_4bit_refuses():
             (lambda: ops.gemv_mx_w4(q, sq, w4, sw), "on the ROCm device")):
         with pytest.raises(RuntimeError, match=why):
             bad()
+
+
+# ---- sampling --------------------------------------------------------------
+
+def _sample64(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """The definition, row by row in 64 bits, and for each row how near a
+    border decided: the smallest distance of a running weight from a border,
+    relative to the row's weight."""
+    rows = logits.shape[0]
+
+    def of(v, i):
+        return v[i].item() if torch.is_tensor(v) else v
+
+    out, near = [], []
+    for i in range(rows):
+        x = logits[i].double().cpu()
+        x = torch.where(x.isnan(), -torch.inf, x)
+        t, k, p, q = (of(v, i) for v in (temperature, top_k, top_p, min_p))
+        s, at = torch.sort(x, descending=True, stable=True)
+        if s[0] == -torch.inf or not t > 0:
+            out.append(-1 if s[0] == -torch.inf else int(at[0]))
+            near.append(1.0)
+            continue
+        w = torch.where(s == s[0], 1.0, torch.exp((s - s[0]) / t))
+        if k >= 1:
+            w = w[:k]
+        c = w.cumsum(0)
+        n, gap = len(w), 1.0
+        if p < 1:
+            n = min(n, int((c - w < p * c[-1]).sum()))
+            gap = float((c - p * c[-1]).abs().min() / c[-1])
+        if q > 0:
+            gap = min(gap, float((w - q)[w != 1.0].abs().min()) if bool((w != 1.0).any()) else 1.0)
+        n = max(1, min(n, int((w >= q).sum())))
+        c = c[:n]
+        want = float(of(u, i)) * float(c[-1])
+        out.append(int(at[min(int((c <= want).sum()), n - 1)]))
+        near.append(min(gap, float((c - want).abs().min() / c[-1])))
+    return torch.tensor(out), torch.tensor(near)
+
+
+# A weight is off by half of 2^-45 and 2^-44 of itself: over V <= 2^17 of them
+# (1 or more in all) a running weight by less than 2^17 * 2^-46 + 2^-44 of the
+# row's. A row whose border is nearer than twice that may go to either side.
+SAMPLE_NEAR = 2 * (2.0 ** -29 + 2.0 ** -44)
+
+
+def _same_tokens(got, logits, u, **settings):
+    want, near = _sample64(logits, u, **settings)
+    far = near > SAMPLE_NEAR
+    return bool((got.cpu().flatten()[far] == want[far]).all()) and bool(far.any())
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.3), dict(temperature=5.0),
+            dict(top_k=1), dict(top_k=7), dict(top_k=1000), dict(top_k=10 ** 9),
+            dict(top_p=0.0), dict(top_p=0.5), dict(top_p=0.97), dict(min_p=0.02),
+            dict(min_p=1.0), dict(temperature=0.7, top_k=40, top_p=0.9, min_p=0.01),
+            dict(temperature=1.4, top_k=3000, top_p=0.99)]
+
+
+def _uniform(rows, seed):
+    return torch.rand(rows, generator=_gen(seed)).to(DEV)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("settings", SETTINGS)
+@pytest.mark.parametrize("rows,v", [(1, 1), (2, 2), (5, 63), (3, 1000), (4, 4097),
+                                    (7, 50001), (2, 131072)])
+def test_sample(rows, v, dtype, settings):
+    x = _randn((rows, v), 50 + v, dtype, 2.5)
+    u = _uniform(rows, 51)
+    got = ops.sample(x, u, **settings)
+    assert got.dtype == torch.int64 and got.shape == (rows,)
+    assert _same_tokens(got, x, u, **settings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_sample_settings_of_each_row(dtype):
+    rows, v = 60, 9001
+    x = _randn((rows, v), 52, dtype, 3.0)
+    g = _gen(53)
+    st = dict(temperature=torch.rand(rows, generator=g) * 2 * (torch.rand(rows, generator=g) > 0.2),
+              top_k=torch.randint(-1, 300, (rows,), generator=g),
+              top_p=0.5 + torch.rand(rows, generator=g).double(),
+              min_p=torch.rand(rows, generator=g) * 0.1)
+    st = {k: t.to(DEV) for k, t in st.items()}
+    u = _uniform(rows, 54)
+    got = ops.sample(x, u, **st)
+    assert _same_tokens(got, x, u, **st)
+    assert torch.equal(got, ops.sample(x, u.double(), **dict(st, top_k=st["top_k"].int())))
+    # alone or among others, a row gives the same
+    for i in (0, 17, 59):
+        one = ops.sample(x[i:i + 1], u[i:i + 1], **{k: t[i:i + 1] for k, t in st.items()})
+        assert int(one) == int(got[i])
+
+
+@gpu
+@pytest.mark.parametrize("v", [100, 5000, 70000])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=30), dict(top_k=5000), dict(top_p=0.4),
+                                      dict(top_k=4999, top_p=0.8), dict(min_p=0.5)])
+def test_sample_ties(v, settings):
+    # all equal; two values; a few values: the lowest indices are kept
+    one = torch.full((v,), 1.5)
+    two = torch.where(torch.arange(v) % 3 == 0, 2.0, 1.0)
+    few = (torch.arange(v) * 7919 % 5).float()
+    zero = torch.where(torch.arange(v) % 2 == 0, 0.0, -0.0)
+    x = torch.stack([one, two, few, zero] * 4).to(DEV)
+    u = torch.linspace(0.013, 0.987, 16).to(DEV)
+    got = ops.sample(x, u, **settings)
+    assert _same_tokens(got, x, u, **settings)
+
+
+@gpu
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=50), dict(top_p=0.9), dict(temperature=0.0),
+                                      dict(temperature=1e-3), dict(temperature=1e4, top_p=0.3)])
+def test_sample_masked_and_extreme_rows(settings):
+    v = 20000
+    x = _randn((10, v), 55, scale=3.0)
+    inf = float("inf")
+    x[0] = -inf                                   # nothing left
+    x[1] = -inf
+    x[1, 777] = -5.0                              # one left
+    x[2, :19000] = torch.finfo(torch.float32).min  # the type's lowest value
+    x[3, ::2] = float("nan")
+    x[4, 11] = x[4, 19999] = inf                  # two infinite
+    x[5] = torch.finfo(torch.float32).min
+    x[6, 5], x[6, 6] = 3e38, -3e38                # a range past f32's
+    x[7] = float("nan")
+    x[8, :] = -inf
+    x[8, 100:400] = torch.randn(300, generator=_gen(56)).to(DEV)
+    x[9] = x[9] * 1e-30                           # all but equal
+    u = torch.linspace(0.05, 0.95, 10).to(DEV)
+    got = ops.sample(x, u, **settings)
+    assert _same_tokens(got, x, u, **settings)
+    assert got[0] == -1 and got[7] == -1 and got[1] == 777
+
+
+@gpu
+def test_sample_draws_by_weight():
+    # the ends of u, and the shares of a small row over a grid of it
+    w = torch.tensor([0.1, 0.4, 0.2, 0.3])
+    n = 1000
+    u = ((torch.arange(n) + 0.5) / n).to(DEV)
+    got = ops.sample(w.log().expand(n, 4).to(DEV), u)
+    share = torch.bincount(got.cpu(), minlength=4) / n
+    assert bool(((share - w).abs() <= 1.01 / n).all())
+    x = w.log().expand(4, 4).contiguous().to(DEV)
+    ends = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 0.39], device=DEV)
+    assert ops.sample(x, ends).tolist() == [1, 0, 0, 1]
+
+
+@gpu
+def test_sample_strided_shaped_and_elsewhere():
+    v = 5003
+    buf = _randn((6, v + 40), 57, torch.bfloat16, 3.0)
+    buf[:, v:] = 100.0
+    u = _uniform(6, 58)
+    x = buf[:, :v]
+    want = ops.sample(x.contiguous(), u, top_p=0.9)
+    assert torch.equal(ops.sample(x, u, top_p=0.9), want)
+    assert torch.equal(ops.sample(x.reshape(2, 3, v), u.view(2, 3), top_p=0.9).flatten(), want)
+    assert ops.sample(x[4], u[4], top_p=0.9).shape == () and \
+        int(ops.sample(x[4], u[4], top_p=0.9)) == int(want[4])
+    cols = x.t().contiguous().t()  # tokens apart, rows together
+    assert torch.equal(ops.sample(cols, u, top_p=0.9), want)
+    for off in range(1, 9):  # rows that start anywhere
+        y = torch.empty(6 * v + off, dtype=torch.bfloat16, device=DEV)[off:].view(6, v)
+        y.copy_(x)
+        assert torch.equal(ops.sample(y, u, top_p=0.9), want)
+    assert ops.sample(x[:0], u[:0]).shape == (0,)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.sample(x, u, top_p=0.9)
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_sample_in_two_graphs():
+    x = _randn((9, 30000), 59, torch.bfloat16, 3.0)
+    u = _uniform(9, 60)
+    ops.sample(x, u, top_p=0.9)
+    graphs, outs = [], []
+    for st in (dict(top_p=0.9), dict(top_k=20)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.sample(x, u, **st))
+        graphs.append(g)
+    for i in range(3):
+        x.copy_(_randn((9, 30000), 61 + i, torch.bfloat16, 3.0))
+        u.copy_(_uniform(9, 70 + i))
+        for g in graphs:
+            g.replay()
+        want = [ops.sample(x, u, top_p=0.9), ops.sample(x, u, top_k=20)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@gpu
+def test_sample_a_long_row():
+    # more chunks than a wave has lanes, and bins that no list holds
+    v = 3_000_001
+    x = _randn((1, v), 62, torch.float32, 2.0)
+    for st in (dict(), dict(top_k=100000), dict(top_p=0.99), dict(temperature=0.0)):
+        u = _uniform(1, 63)
+        got = ops.sample(x, u, **st)
+        want, _ = _sample64(x, u, **st)
+        assert int(got) == int(want)
+
+
+@built
+def test_sample_refuses():
+    x, u = torch.zeros(3, 10), torch.zeros(3)
+    for bad, why in (
+            (lambda: ops.sample(x.long(), u), "supports bf16"),
+            (lambda: ops.sample(x, u[:2]), "u must have one value"),
+            (lambda: ops.sample(x, u.half()), "f32 or f64"),
+            (lambda: ops.sample(x, u.view(3, 1)), "one value for each row"),
+            (lambda: ops.sample(x, u, temperature=-1.0), "temperature must be"),
+            (lambda: ops.sample(x, u, temperature=float("nan")), "temperature must be"),
+            (lambda: ops.sample(x, u, temperature=float("inf")), "temperature must be"),
+            (lambda: ops.sample(x, u, top_k=-1), "top_k must be"),
+            (lambda: ops.sample(x, u, top_p=1.5), "top_p must be"),
+            (lambda: ops.sample(x, u, min_p=-0.1), "min_p must be"),
+            (lambda: ops.sample(x, u, top_k=torch.zeros(3)), "int32 or int64"),
+            (lambda: ops.sample(x, u, top_p=torch.zeros(3).int()), "f32 or f64"),
+            (lambda: ops.sample(x, u, top_p=torch.zeros(2)), "one value for each row"),
+            (lambda: ops.sample(torch.zeros(3, 0), u), "V >= 1"),
+            (lambda: ops.sample(torch.tensor(1.0), u), "expects logits"),
+            (lambda: ops.sample(x, u), "on the ROCm device")):
+        with pytest.raises(RuntimeError, match=why):
+            bad()
