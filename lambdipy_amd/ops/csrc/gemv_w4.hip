@@ -3,17 +3,24 @@
 //   y[m, n] = sum_k x[m, k] * e2m1(w[n, k]) * 2^(sw[n, k/32] - 127)
 //
 // x in bf16 or fp16, or MX e4m3 with scales of its own. What has to move is
-// the weights (0.53 B an element), so they go from memory straight into the
-// registers of the one wave that multiplies them. The products are taken by
-// the 16-bit MFMA with f32 sums: e2m1 and e4m3 values times their power of
-// two are exact in bf16, and so is every product in f32. (The scaled
-// f8f6f4 MFMA would take the bytes as they are, but does not hold its inner
-// sums to f32: 2.7e-5 off over K = 512.)
+// the weights (0.53 B an element). The products are taken by the 16-bit MFMA
+// with f32 sums: e2m1 and e4m3 values times their power of two are exact in
+// bf16, and so is every product in f32. (The scaled f8f6f4 MFMA would take
+// the bytes as they are, but does not hold its inner sums to f32: 2.7e-5 off
+// over K = 512.)
 //
-// A wave takes 128 k a step of 16 weight rows a tile: lane (c, g) =
-// (lane & 15, lane >> 4) loads the 16 B of row c's block g. The waves of a
+// A wave takes 128 k a step: 16 rows of weights a tile, 16 rows of x a tile.
+// The MFMA wants neighbouring lanes in different rows, the load path
+// neighbouring lanes in one row (16 clocks a load of 1 KB then, 64
+// otherwise, which bound everything but the smallest x), so each wave turns
+// its steps round through LDS of its own, without a barrier. The waves of a
 // workgroup split K step by step, so that together they read neighbouring
 // bytes of a row, and join their sums in LDS in a fixed order.
+//
+// Measured: 100000 x 8192 by one bf16 row 73 us, 5.9 TB/s (reading alone
+// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.4 us; 28000 x 8192 by 64
+// MX rows 44 us, where the MFMA (27% busy) and the conversions to bf16 take
+// more than the memory.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -93,75 +100,93 @@ __device__ __forceinline__ i32x4 transpose_groups(i32x4 r) {
   return i32x4{(int)c[0], (int)c[1], (int)d[0], (int)d[1]};
 }
 
-// What one step of a wave multiplies.
-template <int MODE, int MT, int NT>
+// What a wave loads for one step, in the order of memory: neighbouring lanes
+// hold neighbouring 16-B pieces of a row.
+// FEW: of x only the rows that one load holds (4, of MX 8) are there.
+template <int MODE, int MT, int NT, bool FEW>
 struct Step {
-  static constexpr int XW = MODE == X_MX ? 2 : 4;  // 16-B loads a row
+  static constexpr int XL = FEW ? 1 : MODE == X_MX ? 2 : 4;  // loads a tile of x
   i32x4 w[NT];
-  unsigned sw[NT];
-  i32x4 x[MT][XW];
-  unsigned sx[MT];
+  i32x4 x[MT][XL];
+  unsigned sw, sx;  // of column, row `lane`
+};
+
+// Where a wave brings a step into the MFMA's order. The pieces of a row are
+// permuted by the row, so that both the writes (along rows) and the reads
+// (down 16 rows) meet every bank once.
+template <int MODE, int MT, int NT, bool FEW>
+struct Exchange {
+  static constexpr int XTILE = Step<MODE, MT, NT, FEW>::XL * 1024;
+  static constexpr int XTILES = MT < 2 ? MT : 2;  // taken in turn
+  static_assert(NT <= 4 && MT <= 4, "a lane brings one scale of each side");
+  unsigned char w[NT][1024];
+  unsigned char x[XTILES][XTILE];
+  unsigned sw[NT * 16], sx[MT * 16];
 };
 
 // MT x NT tiles of 16 rows of x by 16 rows of weights.
-template <int MODE, int MT, int NT, int WAVES, int DEPTH>
+template <int MODE, int MT, int NT, int WAVES, int DEPTH, bool FEW>
 __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
-  typedef Step<MODE, MT, NT> S;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  static_assert(!FEW || MT == 1, "few rows are one tile");
+  typedef Step<MODE, MT, NT, FEW> S;
+  typedef Exchange<MODE, MT, NT, FEW> E;
+  __shared__ union Shared {
+    E exchange[WAVES];
+    f32x4 part[WAVES][MT * NT][64];
+    __device__ Shared() {}
+  } sh;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * NT * 16, m0 = (int)blockIdx.y * MT * 16;
+  const int xc = FEW ? c & (MODE == X_MX ? 7 : 3) : c;
+  // neighbouring tiles on one XCD: their scales share lines of its L2
+  const int n0 = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x) * NT * 16;
+  const int m0 = (int)blockIdx.y * MT * 16;
   const int steps = (a.K + 127) >> 7;
   const bool half_last = (a.K & 127) != 0;
+  E& ex = sh.exchange[wave];
 
   // Rows behind the last are the last again; their sums are not stored.
-  const unsigned char* wp[NT];
-  const unsigned char* swp[NT];
-  const unsigned char* xp[MT];
-  const unsigned char* sxp[MT];
+  constexpr int WROW = 4;                        // pieces of a row a step
+  constexpr int XROW = MODE == X_MX ? 8 : 16;
+  const unsigned char* const w0 = a.w + (long)n0 * (a.K >> 1);
+  const unsigned char* const x0 = a.x + m0 * a.x_stride;
+  unsigned woff[NT], xoff[MT][S::XL];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int n = min(n0 + t * 16 + c, a.N - 1);
-    wp[t] = a.w + (long)n * (a.K >> 1) + g * 16;
-    swp[t] = a.sw + (long)n * 4;
-  }
+  for (int t = 0; t < NT; ++t)
+    woff[t] = (unsigned)min(t * 16 + lane / WROW, a.N - 1 - n0) * (unsigned)(a.K >> 1) +
+              lane % WROW * 16;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = min(m0 + t * 16 + c, a.M - 1);
-    xp[t] = a.x + m * a.x_stride +
-            (MODE == X_BF16 ? g * 64 : MODE == X_F16 ? g * 16
-                                                     : (g >> 1) * 64 + (g & 1) * 16);
-    sxp[t] = MODE == X_MX ? a.sx + (long)m * 4 : nullptr;
-  }
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int l = 0; l < S::XL; ++l)
+      xoff[i][l] = (unsigned)min(i * 16 + l * (64 / XROW) + lane / XROW, a.M - 1 - m0) *
+                       (unsigned)a.x_stride + lane % XROW * 16;
+  const unsigned swoff = (unsigned)min(lane % (NT * 16), a.N - 1 - n0) * 4;
+  const unsigned sxoff = (unsigned)min(lane % (MT * 16), a.M - 1 - m0) * 4;
 
-  auto load = [&](S& f, int s) {
-    // K may end after the first two blocks of the last step
+  // Turn i of a wave is step wave + i * WAVES. Loads are issued without a
+  // branch, so that the compiler's waits count them: turns behind the last
+  // step read that one again, and where K ends in the middle of the last
+  // step, the second half of the pieces reads the first half again.
+  // `multiply` clears what was read in place of nothing.
+  const int turns = (steps + WAVES - 1) / WAVES;
+  auto load = [&](S& f, int turn) {
+    const int s = min(wave + turn * WAVES, steps - 1);
     const bool half = half_last && s == steps - 1;
-    const bool in = !half || g < 2;
-    const i32x4 zero = {0, 0, 0, 0};
+    const unsigned wback = half && lane % WROW >= WROW / 2 ? WROW / 2 * 16 : 0;
+    const unsigned xback = half && lane % XROW >= XROW / 2 ? XROW / 2 * 16 : 0;
+    const unsigned char* const w = w0 + (long)s * (WROW * 16);
+    const unsigned char* const x = x0 + (long)s * (XROW * 16);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      f.w[t] = in ? load16(wp[t] + (long)s * 64) : zero;
-      f.sw[t] = load4(swp[t] + (long)s * a.N * 4);
-      if (half) f.sw[t] &= 0xffffu;
-    }
+    for (int t = 0; t < NT; ++t) f.w[t] = load16(w + (woff[t] - wback));
+    f.sw = load4(a.sw + ((long)s * a.N + n0) * 4 + swoff);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if constexpr (MODE == X_MX) {
-        f.x[t][0] = in ? load16(xp[t] + (long)s * 128) : zero;
-        f.x[t][1] = in ? load16(xp[t] + (long)s * 128 + 32) : zero;
-        f.sx[t] = load4(sxp[t] + (long)s * a.M * 4);
-        if (half) f.sx[t] &= 0xffffu;
-      } else if constexpr (MODE == X_BF16) {
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          f.x[t][j] = in ? load16(xp[t] + (long)s * 256 + j * 16) : zero;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          f.x[t][j] = !half || j < 2 ? load16(xp[t] + (long)s * 256 + j * 64)
-                                     : zero;
-      }
-    }
+      for (int l = 0; l < S::XL; ++l) f.x[i][l] = load16(x + (xoff[i][l] - xback));
+    if constexpr (MODE == X_MX)
+      f.sx = load4(a.sx + ((long)s * a.M + m0) * 4 + sxoff);
   };
 
   f32x4 acc[MT][NT];
@@ -170,49 +195,99 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
 
-  auto multiply = [&](const S& f) {
-    if constexpr (MODE == X_F16) {
-      // fp16 cannot hold every power of two, so here each MFMA takes one
-      // block (its words spread over the lane groups) and the block's scale
-      // goes onto the sum.
+  auto put = [](unsigned char* p, i32x4 v) { *reinterpret_cast<i32x4*>(p) = v; };
+  auto get = [](const unsigned char* p) { return *reinterpret_cast<const i32x4*>(p); };
+  // A wave's LDS operations are carried out in order; this keeps the
+  // compiler to it.
+  auto in_order = [] {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto wat = [](int row, int piece) { return (row * 4 + (piece ^ (row >> 2))) * 16; };
+  auto xat = [](int row, int piece) {
+    return MODE == X_MX ? (row * 8 + (piece ^ (row >> 1))) * 16
+                        : (row * 16 + (piece ^ row)) * 16;
+  };
+
+  auto multiply = [&](const S& f, int turn) {
+    const int s = wave + turn * WAVES;
+    const bool none = s >= steps;
+    const bool part = none || (half_last && s == steps - 1);
+    const i32x4 zero = {0, 0, 0, 0};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const i32x4 w = transpose_groups(f.w[t]);
+    for (int t = 0; t < NT; ++t) put(ex.w[t] + wat(lane / WROW, lane % WROW), f.w[t]);
+    ex.sw[lane % (NT * 16)] = part ? f.sw & 0xffffu : f.sw;
+    if constexpr (MODE == X_MX)
+      ex.sx[lane % (MT * 16)] = part ? f.sx & 0xffffu : f.sx;
+    in_order();
+    i32x4 w[NT];
+    unsigned sw[NT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const nf16x8 b = w_f16(w[j]);
-          const float s = scale_of(f.sw[t], j);
+    for (int t = 0; t < NT; ++t) {
+      w[t] = get(ex.w[t] + wat(c, g));
+      sw[t] = ex.sw[t * 16 + c];
+      if (part && (none || g >= 2)) w[t] = zero;
+    }
+    // 16-bit weights, once for all rows of x
+    i32x4 b[NT][4];
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(nf16x8, f.x[i][j]), b, f32x4{0, 0, 0, 0}, 0,
-                0, 0);
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (MODE == X_F16) w[t] = transpose_groups(w[t]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[i][t][r] = __builtin_fmaf(p[r], s, acc[i][t][r]);
-          }
-        }
+      for (int j = 0; j < 4; ++j)
+        b[t][j] = MODE == X_F16
+                      ? __builtin_bit_cast(i32x4, w_f16(w[t][j]))
+                      : __builtin_bit_cast(i32x4, w_bf16(w[t][j], scale_of(sw[t], g)));
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      unsigned char* const xs = ex.x[i % E::XTILES];
+#pragma unroll
+      for (int l = 0; l < S::XL; ++l)
+        put(xs + xat(l * (64 / XROW) + lane / XROW, lane % XROW), f.x[i][l]);
+      in_order();
+      i32x4 x[4];
+      if constexpr (MODE == X_MX) {
+        // a lane's block lies in the pieces of two quarters
+        const int q = (g >> 1) * 4 + (g & 1);
+        const i32x4 lo = get(xs + xat(xc, q)), hi = get(xs + xat(xc, q + 2));
+        const float sx = scale_of(ex.sx[i * 16 + c], g);
+        x[0] = __builtin_bit_cast(i32x4, x_bf16(lo[0], lo[1], sx));
+        x[1] = __builtin_bit_cast(i32x4, x_bf16(lo[2], lo[3], sx));
+        x[2] = __builtin_bit_cast(i32x4, x_bf16(hi[0], hi[1], sx));
+        x[3] = __builtin_bit_cast(i32x4, x_bf16(hi[2], hi[3], sx));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[j] = get(xs + xat(xc, MODE == X_F16 ? 4 * j + g : 4 * g + j));
       }
-    } else {
-      // MFMA j takes elements [8j, 8j+8) of the four groups' blocks
+      if (part) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (none || (MODE == X_F16 ? j >= 2 : g >= 2)) x[j] = zero;
+      }
+      in_order();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        nbf16x8 x[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          if constexpr (MODE == X_BF16)
-            x[i] = __builtin_bit_cast(nbf16x8, f.x[i][j]);
-          else
-            x[i] = x_bf16(f.x[i][j >> 1][(j & 1) * 2],
-                          f.x[i][j >> 1][(j & 1) * 2 + 1], scale_of(f.sx[i], g));
-        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const nbf16x8 b = w_bf16(f.w[t][j], scale_of(f.sw[t], g));
+          if constexpr (MODE == X_F16) {
+            // fp16 cannot hold every power of two, so here each MFMA takes
+            // one block (its words spread over the lane groups) and the
+            // block's scale goes onto the sum
+            const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                __builtin_bit_cast(nf16x8, x[j]), __builtin_bit_cast(nf16x8, b[t][j]),
+                f32x4{0, 0, 0, 0}, 0, 0, 0);
+            const float sc = scale_of(sw[t], j);
 #pragma unroll
-          for (int i = 0; i < MT; ++i)
+            for (int r = 0; r < 4; ++r)
+              acc[i][t][r] = __builtin_fmaf(p[r], sc, acc[i][t][r]);
+          } else {
+            // MFMA j takes elements [8j, 8j+8) of the four groups' blocks
             acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                x[i], b, acc[i][t], 0, 0, 0);
+                __builtin_bit_cast(nbf16x8, x[j]), __builtin_bit_cast(nbf16x8, b[t][j]),
+                acc[i][t], 0, 0, 0);
+          }
         }
       }
     }
@@ -220,31 +295,31 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
 
   S f[DEPTH];
 #pragma unroll
-  for (int d = 0; d < DEPTH; ++d)
-    if (wave + d * WAVES < steps) load(f[d], wave + d * WAVES);
-  for (int s = wave; s < steps; s += DEPTH * WAVES) {
+  for (int d = 0; d < DEPTH; ++d) load(f[d], d);
+  int turn = 0;
+  for (; turn + DEPTH < turns; turn += DEPTH) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const int now = s + d * WAVES;
-      if (now < steps) {
-        multiply(f[d]);
-        if (now + DEPTH * WAVES < steps) load(f[d], now + DEPTH * WAVES);
-      }
+      multiply(f[d], turn + d);
+      load(f[d], turn + d + DEPTH);
     }
   }
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d)
+    if (turn + d < turns) multiply(f[d], turn + d);
 
   // Join the waves' sums; then a thread owns four rows of one column.
-  __shared__ f32x4 part[WAVES][MT * NT][64];
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) part[wave][i * NT + t][lane] = acc[i][t];
+    for (int t = 0; t < NT; ++t) sh.part[wave][i * NT + t][lane] = acc[i][t];
   __syncthreads();
   for (int e = (int)threadIdx.x; e < MT * NT * 64; e += WAVES * 64) {
     const int tile = e >> 6, l = e & 63;
-    f32x4 v = part[0][tile][l];
+    f32x4 v = sh.part[0][tile][l];
 #pragma unroll
-    for (int k = 1; k < WAVES; ++k) v += part[k][tile][l];
+    for (int k = 1; k < WAVES; ++k) v += sh.part[k][tile][l];
     const int n = n0 + (tile % NT) * 16 + (l & 15);
     const int m = m0 + (tile / NT) * 16 + (l >> 4) * 4;
     if (n >= a.N) continue;
@@ -260,22 +335,42 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
   }
 }
 
-template <int MODE, int MT, int NT, int WAVES, int DEPTH>
+template <int MODE, int MT, int NT, int WAVES, int DEPTH, bool FEW = false>
 hipError_t launch(const W4Args& a, hipStream_t stream) {
   const dim3 grid((unsigned)((a.N + NT * 16 - 1) / (NT * 16)),
                   (unsigned)((a.M + MT * 16 - 1) / (MT * 16)));
-  gemv_w4_kernel<MODE, MT, NT, WAVES, DEPTH>
+  gemv_w4_kernel<MODE, MT, NT, WAVES, DEPTH, FEW>
       <<<grid, dim3(WAVES * 64), 0, stream>>>(a);
   return hipGetLastError();
 }
 
+// The largest tile whose workgroups still fill the chip: a wave loads x once
+// for all the weight rows of its tile, so that wide tiles cost less a weight,
+// but with fewer than one workgroup a CU the rest of the chip is idle. Over
+// M = 12 .. 64 and N x K from 1000 x 2048 to 100000 x 8192 this is the
+// fastest of the sixteen shapes tried or within a tenth of it (8192 x 8192,
+// M = 64 MX: 32 x 64 tiles on 256 workgroups 15.0 us, 64 x 64 on 128 more
+// than 19.6; 28000 x 8192: 56 and 44 us).
 template <int MODE>
 hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
-  if (a.K < 64 || a.K % 64 != 0) return hipErrorInvalidValue;
-  if (a.M <= 16) return launch<MODE, 1, 1, 8, 2>(a, stream);
-  if (a.M <= 32) return launch<MODE, 2, 2, 8, 2>(a, stream);
-  return launch<MODE, 4, 2, 4, 2>(a, stream);
+  if (a.K < 64 || a.K % 64 != 0 || a.K > (1 << 24)) return hipErrorInvalidValue;
+  constexpr long CUS = 256;
+  auto fills = [&](int mt, int nt) {
+    return (long)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)) >= CUS;
+  };
+  // Rows that one load of x holds: 100000 x 8192 by one bf16 row 73 us,
+  // loading a tile of 16 rows of x 80 us.
+  if (a.M <= (MODE == X_MX ? 8 : 4))
+    return fills(1, 2) ? launch<MODE, 1, 2, 8, 2, true>(a, stream)
+                       : launch<MODE, 1, 1, 8, 2, true>(a, stream);
+  if constexpr (MODE != X_F16)  // whose scaled sums do not fit the registers
+    if (a.M > 32 && fills(4, 4)) return launch<MODE, 4, 4, 4, 1>(a, stream);
+  if (a.M > 16 && fills(2, 4)) return launch<MODE, 2, 4, 8, 1>(a, stream);
+  if (a.M > 16 && fills(2, 2)) return launch<MODE, 2, 2, 8, 1>(a, stream);
+  if (fills(1, 4)) return launch<MODE, 1, 4, 8, 1>(a, stream);
+  if (fills(1, 2)) return launch<MODE, 1, 2, 8, 1>(a, stream);
+  return launch<MODE, 1, 1, 8, 1>(a, stream);
 }
 
 }  // namespace

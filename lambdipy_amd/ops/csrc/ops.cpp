@@ -875,7 +875,7 @@ void check_w4(const at::Tensor& w, const at::Tensor& sw, int64_t K, const char* 
               ": scale shapes must be [ceil(K/128), rows, 4] (tile-major)");
   TORCH_CHECK(w.is_contiguous() && sw.is_contiguous(), what,
               ": weights and scales must be contiguous");
-  TORCH_CHECK(K <= (1 << 30) && w.size(0) <= (1 << 30), what, ": too large");
+  TORCH_CHECK(K <= (1 << 24) && w.size(0) <= (1 << 30), what, ": too large");
 }
 
 at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor& sB,
@@ -890,7 +890,9 @@ at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor&
   TORCH_CHECK(Bt4.device() == x.device() && sB.device() == x.device(),
               "gemv_w4: all tensors must be on one device");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-  const at::Tensor rows = dense_rows(x);
+  at::Tensor rows = dense_rows(x);
+  // the kernel's offsets within a tile of rows are 32 bits
+  if (rows.stride(0) > (1 << 24)) rows = rows.contiguous();
   auto sizes = x.sizes().vec();
   sizes.back() = N;
   auto y = at::empty(sizes, x.options()
