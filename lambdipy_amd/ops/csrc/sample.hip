@@ -31,6 +31,7 @@ constexpr int CHUNK_THREADS = 256;
 constexpr int ROW_THREADS = 1024;
 constexpr int LIST = 4096;  // members of bins kept in LDS
 constexpr int FEW = 64;     // members that one wave ranks
+constexpr int WHOLE = 65536;  // rows up to here are one workgroup's
 
 struct ChunkMax {
   float hi, lo;  // largest; smallest that is not -inf
@@ -67,21 +68,17 @@ __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float as_f32(__bf16 x) { return (float)x; }
 
-// f(index, logit) for every logit of [begin, end) that a token can be drawn
-// from: not NaN, not -inf. A thread's indices rise.
+// f(index, logit) for every logit of [begin, end). A thread's indices rise.
 // AHEAD: 16-B loads in flight a thread.
 template <int THREADS, int AHEAD, typename T, typename F>
 __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
                                      int end, F f) {
   constexpr int VEC = 16 / sizeof(T);
   typedef T V __attribute__((ext_vector_type(VEC)));
-  auto one = [&](int i, float x) {
-    if (x > -__builtin_inff()) f(i, x + 0.f);  // -0 is 0
-  };
   const int tid = (int)threadIdx.x;
   const int off = (int)(((uintptr_t)(row + begin) & 15) / sizeof(T));
   const int head = min(off ? VEC - off : 0, end - begin);
-  if (tid < head) one(begin + tid, as_f32(row[begin + tid]));
+  if (tid < head) f(begin + tid, as_f32(row[begin + tid]));
   const int first = begin + head;
   const int vecs = (end - first) / VEC;
   const V* body = reinterpret_cast<const V*>(row + first);
@@ -95,23 +92,17 @@ __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
       if (i + a * THREADS >= vecs) break;
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
-        one(first + (i + a * THREADS) * VEC + j, as_f32(v[a][j]));
+        f(first + (i + a * THREADS) * VEC + j, as_f32(v[a][j]));
     }
   }
   const int tail = first + vecs * VEC + tid;
-  if (tail < end) one(tail, as_f32(row[tail]));
+  if (tail < end) f(tail, as_f32(row[tail]));
 }
 
 // ---- a row's weights and bins --------------------------------------------
 
-struct RowScale {
-  float hi;       // the row's largest logit
-  double inv_t;
-  double one;     // 2^shift
-  float per_bin;  // bins per unit of x
-  int at;
-  bool greedy;
-};
+// A token can be drawn from this logit: it is not -inf and not NaN.
+__device__ __forceinline__ bool real(float x) { return x > -__builtin_inff(); }
 
 // The largest logit with its lowest index, and the smallest.
 struct Extent {
@@ -131,44 +122,89 @@ struct Extent {
   }
 };
 
-// Every wave works it out for itself: the same bits in every kernel.
-__device__ __forceinline__ RowScale row_scale(const SampleArgs& a, int row) {
+struct RowScale {
+  float hi;       // the row's largest logit
+  float per_bin;  // bins per unit of x
+  double hi64;    // a number over f32's where that is infinite
+  double per_x;   // powers of two per unit of x
+  double shift;
+  int at;
+  bool greedy, by_k, by_p;
+};
+
+constexpr double INFINITE = 1e300;
+
+__device__ __forceinline__ RowScale row_scale(const SampleArgs& a, int row,
+                                              Extent e) {
 #pragma clang fp contract(off)
+  RowScale r;
+  r.hi = e.hi;
+  r.hi64 = fmin((double)e.hi, INFINITE);
+  r.at = e.hi > -__builtin_inff() ? e.at : -1;
+  const double t = param(a.temperature, row);
+  r.greedy = !(t > 0) || r.at < 0;
+  r.by_k = param(a.top_k, row) >= 1;
+  r.by_p = param(a.top_p, row) < 1;
+  r.per_x = fmin(1.4426950408889634 / t, 1e300);  // 1 / (T ln 2)
+  r.shift = a.shift;
+  // Below 32 T the weight rounds to nothing (e^-32 < 2^-46). A range that is
+  // nothing or infinite is one bin.
+  const double reach = fmin((double)e.hi - (double)e.lo, 32.0 * t);
+  const double per = BINS / reach;
+  r.per_bin = !(reach > 0) || e.hi == __builtin_inff() ? 0.f
+              : per < 1e30                             ? (float)per
+                                                       : 1e30f;
+  return r;
+}
+
+// The row's extent from its chunks': every wave works it out for itself.
+__device__ __forceinline__ Extent row_extent(const SampleArgs& a, int row) {
   const ChunkMax* c = a.maxima + (long)row * a.chunks;
   Extent e;
   for (int i = (int)threadIdx.x & 63; i < a.chunks; i += 64)
     e.join(c[i].hi, c[i].lo, c[i].at);
   e.join_wave();
-  const float lo = e.lo;
-  RowScale r;
-  r.hi = e.hi;
-  r.at = e.hi > -__builtin_inff() ? e.at : -1;
-  const double t = param(a.temperature, row);
-  r.greedy = !(t > 0) || r.at < 0;
-  r.inv_t = 1.0 / t;
-  r.one = __builtin_ldexp(1.0, a.shift);
-  // Below 32 T the weight rounds to nothing (e^-32 < 2^-46).
-  const double reach = fmin((double)r.hi - (double)lo, 32.0 * t);
-  const double per = BINS / reach;
-  r.per_bin = reach > 0 && per < 1e30 ? (float)per : reach > 0 ? 1e30f : 0.f;
-  return r;
+  return e;
 }
 
 __device__ __forceinline__ int bin_of(const RowScale& r, float x) {
 #pragma clang fp contract(off)
-  // monotone in x; infinities and 0 * inf end in the last bin
-  const float d = x == r.hi ? 0.f : r.hi - x;
-  return (int)fminf(d * r.per_bin, (float)(BINS - 1));
+  // falls as x rises; 0 * inf ends in the last bin
+  return (int)fminf((r.hi - x) * r.per_bin, (float)(BINS - 1));
 }
 
-// The same bits wherever it is inlined: nothing here may be contracted in
-// one place and not in another.
+// a * b + c in one instruction. (From the builtin the compiler makes the
+// two-address form and a move for every constant.)
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
+}
+
+// 2^shift * exp((x - hi) / T), rounded; 0 of -inf and NaN. The same bits
+// wherever it is inlined: nothing here is contracted in one place and not in
+// another.
 __device__ __forceinline__ u64 weight(const RowScale& r, float x) {
 #pragma clang fp contract(off)
-  if (x == r.hi) return (u64)r.one;
-  const double t = ((double)x - (double)r.hi) * r.inv_t;
-  const double w = exp(t) * r.one;
-  return w > 0 ? (u64)(w + 0.5) : 0;
+  const double d = fmin((double)x, INFINITE) - r.hi64;
+  // 2^-2 and less rounds to nothing; fmax takes the number of the two
+  const double y = fmax(__builtin_fma(d, r.per_x, r.shift), -2.0);
+  const double n = __builtin_rint(y), f = y - n;
+  // (2^f - 1) / f on [-1/2, 1/2], the polynomial of degree 8 through nine
+  // Chebyshev nodes: 2^f is off by 2^-44.6 of itself at most
+  double p = 1.0203121156603192e-07;
+  p = fma_const(f, p, 1.325522487537687e-06);
+  p = fma_const(p, f, 1.5252686845879443e-05);
+  p = fma_const(p, f, 0.0001540345585246757);
+  p = fma_const(p, f, 0.001333355817904356);
+  p = fma_const(p, f, 0.009618129159402543);
+  p = fma_const(p, f, 0.055504108664760424);
+  p = fma_const(p, f, 0.2402265069581299);
+  p = fma_const(p, f, 0.6931471805599453);
+  p = fma_const(p, f, 1.0);
+  // 2^52 more leaves the rounded integer in the low bits
+  const double w = __builtin_amdgcn_ldexp(p, (int)n) + 0x1p52;
+  return (u64)__builtin_bit_cast(long long, w) & 0xfffffffffffffull;
 }
 
 // ---- 1: maxima ------------------------------------------------------------
@@ -180,7 +216,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_max_kernel(SampleArgs a) 
   const int end = min(begin + a.chunk, a.vocab);
   Extent e;
   scan<CHUNK_THREADS, 2>(static_cast<const T*>(a.logits) + row * a.stride, begin,
-                         end, [&](int i, float x) { e.join(x, x, i); });
+                         end, [&](int i, float x) {
+                           e.join(x, real(x) ? x : e.lo, i);
+                         });
   e.join_wave();
   __shared__ ChunkMax part[CHUNK_THREADS / 64];
   if ((threadIdx.x & 63) == 0)
@@ -194,29 +232,40 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_max_kernel(SampleArgs a) 
 
 // ---- 2: histograms --------------------------------------------------------
 
+// Adds [begin, end) of a row to bins in LDS. Counts are only asked for where
+// the row is cut by top-k or top-p.
+template <int THREADS, typename T, typename B>
+__device__ __forceinline__ void add_bins(B& b, const RowScale& r, double min_p,
+                                         const T* row, int begin, int end) {
+  const bool counted = r.by_k || r.by_p;
+  const u64 least = (u64)ceil(fmax(0.0, fmin(min_p, 2.0)) * (double)(1ll << (int)r.shift));
+  u64 minp = 0;
+  scan<THREADS, 2>(row, begin, end, [&](int, float x) {
+    const int bin = bin_of(r, x);
+    const u64 w = weight(r, x);
+    if (counted && real(x)) atomicAdd(&b.count[bin], 1u);
+    if (w) atomicAdd(&b.mass[bin], w);
+    minp += w >= least ? w : 0;
+  });
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) minp += __shfl_xor(minp, m, 64);
+  if ((threadIdx.x & 63) == 0) atomicAdd(&b.minp, minp);
+}
+
 template <typename T>
 __global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a) {
   const int row = (int)blockIdx.x / a.chunks;
   const int begin = (int)blockIdx.x % a.chunks * a.chunk;
   const int end = min(begin + a.chunk, a.vocab);
-  const RowScale r = row_scale(a, row);
+  const RowScale r = row_scale(a, row, row_extent(a, row));
   if (r.greedy) return;
   __shared__ ChunkBins b;
   b.mass[threadIdx.x] = 0;
   b.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) b.minp = 0;
   __syncthreads();
-  const double least = param(a.min_p, row) * r.one;
-  u64 minp = 0;
-  scan<CHUNK_THREADS, 2>(static_cast<const T*>(a.logits) + row * a.stride, begin,
-                      end, [&](int, float x) {
-                        const int bin = bin_of(r, x);
-                        const u64 w = weight(r, x);
-                        atomicAdd(&b.count[bin], 1u);
-                        if (w) atomicAdd(&b.mass[bin], w);
-                        if ((double)w >= least) minp += w;
-                      });
-  atomicAdd(&b.minp, minp);
+  add_bins<CHUNK_THREADS>(b, r, param(a.min_p, row),
+                          static_cast<const T*>(a.logits) + row * a.stride, begin, end);
   __syncthreads();
   ChunkBins& out = a.bins[blockIdx.x];
   out.mass[threadIdx.x] = b.mass[threadIdx.x];
@@ -228,7 +277,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a)
 
 // Sorts ascending as (x falling, index rising); no two are equal.
 __device__ __forceinline__ u64 order_of(float x, int i) {
-  const unsigned b = __float_as_uint(x);
+  const unsigned b = __float_as_uint(x + 0.f);  // -0 is 0
   const unsigned up = b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
   return ((u64)~up << 32) | (unsigned)i;
 }
@@ -238,27 +287,34 @@ __device__ __forceinline__ float logit_of(u64 o) {
   return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-struct Bins {
-  u64 mass[BINS];
-  unsigned count[BINS];
+struct Member {
+  u64 order, weight;
 };
 
 struct RowShared {
-  Bins row, sub;  // running sums, bin by bin
+  ChunkBins row, sub;  // running sums, bin by bin
   u64 list[LIST];
-  u64 few[FEW];
+  Member few[FEW];
+  ChunkMax extent[ROW_THREADS / 64];
   u64 wave_mass[BINS / 64];
   unsigned wave_count[BINS / 64];
   u64 lo, hi;
-  u64 minp;
   unsigned n;
-  int bin;
+  int bin, found;
   u64 mass;  // a border's answer
   int at;
 };
 
+__device__ __forceinline__ void clear(ChunkBins& b) {
+  if (threadIdx.x < BINS) {
+    b.mass[threadIdx.x] = 0;
+    b.count[threadIdx.x] = 0;
+  }
+  if (threadIdx.x == 0) b.minp = 0;
+}
+
 // Counts and masses of bins -> running sums.
-__device__ __forceinline__ void run_up(Bins& b, RowShared& sh) {
+__device__ __forceinline__ void run_up(ChunkBins& b, RowShared& sh) {
   const int t = (int)threadIdx.x, lane = t & 63;
   u64 m = 0;
   unsigned c = 0;
@@ -288,15 +344,15 @@ __device__ __forceinline__ void run_up(Bins& b, RowShared& sh) {
     b.mass[t] = m;
     b.count[t] = c;
   }
+  if (t == 0) sh.bin = BINS - 1;
   __syncthreads();
 }
 
 // The first bin whose running sum reaches `border`, which some bin's does.
-__device__ __forceinline__ int bin_at(const Bins& b, bool by_count, u64 border,
-                                      RowShared& sh) {
+// (One thread at most writes sh.bin; it holds some bin from run_up on.)
+__device__ __forceinline__ int bin_at(const ChunkBins& b, bool by_count,
+                                      u64 border, RowShared& sh) {
   const int t = (int)threadIdx.x;
-  if (t == 0) sh.bin = BINS - 1;
-  __syncthreads();
   if (t < BINS) {
     const u64 now = by_count ? b.count[t] : b.mass[t];
     const u64 before = t == 0 ? 0 : by_count ? b.count[t - 1] : b.mass[t - 1];
@@ -316,10 +372,14 @@ struct RowPick {
   RowShared& sh;
   int first = 0, last = -1;  // the bins whose members are in the list
 
+  __device__ __forceinline__ bool listed(int bin) const {
+    return first <= bin && bin <= last;
+  }
+
   // f(order, logit) of the members of `bin` between lo and hi
   template <typename F>
   __device__ __forceinline__ void members(int bin, u64 lo, u64 hi, F f) {
-    if (first <= bin && bin <= last) {
+    if (listed(bin)) {
       const int n = (int)min(sh.n, (unsigned)LIST);
       for (int i = (int)threadIdx.x; i < n; i += ROW_THREADS) {
         const u64 o = sh.list[i];
@@ -328,40 +388,45 @@ struct RowPick {
       }
     } else {
       scan<ROW_THREADS, 1>(row, 0, a.vocab, [&](int i, float x) {
-        if (bin_of(r, x) != bin) return;
+        if (bin_of(r, x) != bin || !real(x)) return;
         const u64 o = order_of(x, i);
         if (lo <= o && o <= hi) f(o, x);
       });
     }
   }
 
-  __device__ __forceinline__ unsigned through(int bin) const {
-    return bin < 0 ? 0 : sh.row.count[bin];
-  }
-
-  // Lists the members of bins [from, to], of which there are at most LIST.
-  __device__ __forceinline__ void collect(int from, int to) {
+  // Lists the members of bins [from, to], unless they are more than LIST.
+  // Returns how many they are.
+  __device__ __forceinline__ unsigned collect(int from, int to) {
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
     scan<ROW_THREADS, 4>(row, 0, a.vocab, [&](int i, float x) {
       const int bin = bin_of(r, x);
-      if (from <= bin && bin <= to) {
+      if (from <= bin && bin <= to && real(x)) {
         const unsigned n = atomicAdd(&sh.n, 1u);
         if (n < LIST) sh.list[n] = order_of(x, i);
       }
     });
     __syncthreads();
     first = from;
-    last = to;
+    last = sh.n <= LIST ? to : from - 1;
+    return sh.n;
   }
 
   // The member of the row at which the running count (mass) reaches `border`:
   // its index to sh.at, the running mass with it to sh.mass.
   __device__ __forceinline__ void resolve(bool by_count, u64 border) {
     const int bin = bin_at(sh.row, by_count, border, sh);
-    unsigned base = through(bin - 1), n = sh.row.count[bin] - base;
+    // what stands before [lo, hi], and how many members that has at most
+    unsigned base = bin ? sh.row.count[bin - 1] : 0;
     u64 mass = bin ? sh.row.mass[bin - 1] : 0;
-    if (!(first <= bin && bin <= last) && n <= LIST) collect(bin, bin);
+    unsigned n;
+    if (listed(bin)) {
+      const unsigned members = sh.row.count[bin] - base;
+      n = first == last ? sh.n : members;
+    } else {
+      n = collect(bin, bin);
+    }
     u64 lo = 0, hi = ~0ull;
     while (n > FEW) {
       // 256 sub-bins between the first and the last member; the two differ,
@@ -370,17 +435,19 @@ struct RowPick {
         sh.lo = ~0ull;
         sh.hi = 0;
       }
-      if (threadIdx.x < BINS) {
-        sh.sub.mass[threadIdx.x] = 0;
-        sh.sub.count[threadIdx.x] = 0;
-      }
+      clear(sh.sub);
       __syncthreads();
       u64 tlo = ~0ull, thi = 0;
       members(bin, lo, hi, [&](u64 o, float) {
         tlo = min(tlo, o);
         thi = max(thi, o);
       });
-      if (tlo <= thi) {
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) {
+        tlo = min(tlo, (u64)__shfl_xor(tlo, m, 64));
+        thi = max(thi, (u64)__shfl_xor(thi, m, 64));
+      }
+      if ((threadIdx.x & 63) == 0 && tlo <= thi) {
         atomicMin(&sh.lo, tlo);
         atomicMax(&sh.hi, thi);
       }
@@ -406,54 +473,91 @@ struct RowPick {
       __syncthreads();
     }
     if (threadIdx.x == 0) {
-      sh.bin = 0;
+      sh.found = 0;
       sh.at = r.at;
       sh.mass = mass;
     }
     __syncthreads();
-    members(bin, lo, hi, [&](u64 o, float) {
-      const int i = atomicAdd(&sh.bin, 1);
-      if (i < FEW) sh.few[i] = o;
+    members(bin, lo, hi, [&](u64 o, float x) {
+      const int i = atomicAdd(&sh.found, 1);
+      if (i < FEW) sh.few[i] = Member{o, weight(r, x)};
     });
     __syncthreads();
     if (threadIdx.x < 64) {
-      const bool mine = threadIdx.x < n;
-      const u64 o = mine ? sh.few[threadIdx.x] : ~0ull;
-      const u64 w = mine ? weight(r, logit_of(o)) : 0;
+      // each lane adds up what is before its member
+      const unsigned found = min(sh.found, FEW);
+      const bool mine = threadIdx.x < found;
+      const Member own = sh.few[mine ? threadIdx.x : 0];
       unsigned before = 0;
       u64 run = 0;
-      for (unsigned j = 0; j < n; ++j) {
-        const u64 oj = __shfl(o, j, 64), wj = __shfl(w, j, 64);
-        if (oj < o) {
-          ++before;
-          run += wj;
-        }
+      for (unsigned j = 0; j < found; ++j) {
+        const Member other = sh.few[j];
+        const bool less = other.order < own.order;
+        before += less;
+        run += less ? other.weight : 0;
       }
-      const u64 now = by_count ? base + before + 1 : mass + run + w;
       const u64 was = by_count ? base + before : mass + run;
+      const u64 now = was + (by_count ? 1 : own.weight);
       if (mine && now >= border && was < border) {
-        sh.mass = mass + run + w;
-        sh.at = (int)(unsigned)o;
+        sh.mass = mass + run + own.weight;
+        sh.at = (int)(unsigned)own.order;
       }
     }
     __syncthreads();
   }
 };
 
+// The borders of a row whose running sums are in sh.row.
+template <typename T>
+__device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
+                                          const RowScale& r, RowShared& sh) {
+  const u64 total = sh.row.mass[BINS - 1];
+  const unsigned all = sh.row.count[BINS - 1];
+  RowPick<T> pick{a, static_cast<const T*>(a.logits) + row * a.stride, r, sh};
+
+  // what a share of a mass has to reach
+  auto share = [](double part, u64 of) {
+    const double s = ceil(part * (double)of);
+    return s >= (double)of ? of : s > 1 ? (u64)s : (u64)1;
+  };
+  u64 kept = total;
+  const double k = param(a.top_k, row);
+  if (r.by_k && k < (double)all) {
+    const unsigned want = (unsigned)k;
+    const int bin = bin_at(sh.row, true, want, sh);
+    if (sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    if (sh.row.count[bin] == want) {
+      kept = sh.row.mass[bin];
+    } else {
+      pick.resolve(true, want);
+      kept = sh.mass;
+    }
+  }
+  if (r.by_p) {
+    const u64 border = share(param(a.top_p, row), kept);
+    const int bin = bin_at(sh.row, false, border, sh);
+    if (!pick.listed(bin) && sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    pick.resolve(false, border);
+    kept = sh.mass;
+  }
+  kept = min(kept, sh.row.minp);
+  const double at = floor(param(a.u, row) * (double)kept);
+  pick.resolve(false, at >= (double)kept ? max(kept, (u64)1)
+                      : at > 0           ? (u64)at + 1
+                                         : (u64)1);
+  return sh.at;
+}
+
 template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   __shared__ RowShared sh;
   const int row = (int)blockIdx.x, t = (int)threadIdx.x;
-  const RowScale r = row_scale(a, row);
+  const RowScale r = row_scale(a, row, row_extent(a, row));
   if (r.greedy) {
     if (t == 0) a.token[row] = r.at;
     return;
   }
-  if (t < BINS) {
-    sh.row.mass[t] = 0;
-    sh.row.count[t] = 0;
-  }
-  if (t == 0) sh.minp = 0;
+  clear(sh.row);
   __syncthreads();
   {
     const ChunkBins* c = a.bins + (long)row * a.chunks;
@@ -466,52 +570,54 @@ __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
     }
     atomicAdd(&sh.row.mass[bin], m);
     atomicAdd(&sh.row.count[bin], n);
-    if (t < a.chunks) atomicAdd(&sh.minp, c[t].minp);
-    for (int i = t + ROW_THREADS; i < a.chunks; i += ROW_THREADS)
-      atomicAdd(&sh.minp, c[i].minp);
+    for (int i = t; i < a.chunks; i += ROW_THREADS)
+      atomicAdd(&sh.row.minp, c[i].minp);
   }
   __syncthreads();
   run_up(sh.row, sh);
+  const int token = pick_token<T>(a, row, r, sh);
+  if (t == 0) a.token[row] = token;
+}
 
-  const u64 total = sh.row.mass[BINS - 1];
-  const unsigned all = sh.row.count[BINS - 1];
-  const double k = param(a.top_k, row), p = param(a.top_p, row);
-  RowPick<T> pick{a, static_cast<const T*>(a.logits) + row * a.stride, r, sh};
-
-  // what a share of a mass has to reach
-  auto share = [](double part, u64 of) {
-    const double s = ceil(part * (double)of);
-    return s >= (double)of ? of : s > 1 ? (u64)s : (u64)1;
-  };
-  u64 kept = total;
-  const bool by_k = k >= 1 && k < (double)all, by_p = p < 1;
-  if (by_k) {
-    const unsigned want = (unsigned)k;
-    const int bin = bin_at(sh.row, true, want, sh);
-    if (sh.row.count[bin] <= LIST) pick.collect(0, bin);
-    if (sh.row.count[bin] == want) {
-      kept = sh.row.mass[bin];
-    } else {
-      pick.resolve(true, want);
-      kept = sh.mass;
-    }
+// All of it in one workgroup, for rows that it reads faster than three
+// kernels follow one another.
+template <typename T>
+__global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
+  __shared__ RowShared sh;
+  const int row = (int)blockIdx.x, t = (int)threadIdx.x;
+  const T* x = static_cast<const T*>(a.logits) + row * a.stride;
+  Extent e;
+  scan<ROW_THREADS, 4>(x, 0, a.vocab, [&](int i, float v) {
+    e.join(v, real(v) ? v : e.lo, i);
+  });
+  e.join_wave();
+  if ((t & 63) == 0) sh.extent[t >> 6] = ChunkMax{e.hi, e.lo, e.at};
+  clear(sh.row);
+  __syncthreads();
+  {
+    const ChunkMax c = sh.extent[t & (ROW_THREADS / 64 - 1)];
+    e.join(c.hi, c.lo, c.at);
+    e.join_wave();
   }
-  if (by_p) {
-    const u64 border = share(p, kept);
-    const int bin = bin_at(sh.row, false, border, sh);
-    if (pick.last < bin && sh.row.count[bin] <= LIST) pick.collect(0, bin);
-    pick.resolve(false, border);
-    kept = sh.mass;
+  const RowScale r = row_scale(a, row, e);
+  if (r.greedy) {
+    if (t == 0) a.token[row] = r.at;
+    return;
   }
-  kept = min(kept, sh.minp);
-  const double at = floor(param(a.u, row) * (double)kept);
-  const u64 border = 1 + (at > 0 ? (at >= (double)kept ? kept - 1 : min((u64)at, kept - 1)) : 0);
-  pick.resolve(false, border);
-  if (t == 0) a.token[row] = sh.at;
+  add_bins<ROW_THREADS>(sh.row, r, param(a.min_p, row), x, 0, a.vocab);
+  __syncthreads();
+  run_up(sh.row, sh);
+  const int token = pick_token<T>(a, row, r, sh);
+  if (t == 0) a.token[row] = token;
 }
 
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  if (a.chunks == 0) {
+    row_whole_kernel<T>
+        <<<dim3((unsigned)a.rows), dim3(ROW_THREADS), 0, stream>>>(a);
+    return hipGetLastError();
+  }
   const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
   chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
   chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
@@ -529,7 +635,8 @@ Plan plan_of(int rows, int vocab) {
   // At least 4096 logits a chunk; more where there are chunks enough for the
   // chip without that, so that fewer histograms are written.
   const long want = ((long)rows * vocab + 2047) / 2048;
-  Plan p;
+  Plan p{};
+  if (vocab <= WHOLE) return p;
   p.chunk = (int)(want < 4096 ? 4096 : (want + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
