@@ -272,8 +272,8 @@ struct SampleParam {
 };
 // token[r]: drawn from row r of logits [rows, vocab] (row stride in elements)
 // by u[r] after temperature, top-k, top-p and min-p; -1 where a row has no
-// logit over -inf. workspace: sample_workspace(rows, vocab) bytes.
-size_t sample_workspace(int rows, int vocab);
+// logit over -inf. workspace: sample_workspace(t, rows, vocab) bytes.
+size_t sample_workspace(ActType t, int rows, int vocab);
 hipError_t sample(ActType t, const void* logits, long stride, int rows,
                   int vocab, SampleParam temperature, SampleParam top_k,
                   SampleParam top_p, SampleParam min_p, SampleParam u,

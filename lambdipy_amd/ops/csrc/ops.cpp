@@ -977,7 +977,7 @@ at::Tensor sample(const at::Tensor& logits, const at::Tensor& u, const Setting& 
   const at::Tensor x = dense_rows(logits);
   auto token = at::empty(logits.sizes().slice(0, logits.dim() - 1),
                          logits.options().dtype(at::kLong));
-  auto work = at::empty({(int64_t)lpx::sample_workspace((int)rows, (int)V)},
+  auto work = at::empty({(int64_t)lpx::sample_workspace(type, (int)rows, (int)V)},
                         logits.options().dtype(at::kByte));
   check_hip(lpx::sample(type, x.data_ptr(), x.stride(0), (int)rows, (int)V, t, k, p, q, draw,
                         work.data_ptr(), token.data_ptr<int64_t>(), current_stream(logits)),

@@ -31,7 +31,8 @@ constexpr int CHUNK_THREADS = 256;
 constexpr int ROW_THREADS = 1024;
 constexpr int LIST = 4096;  // members of bins kept in LDS
 constexpr int FEW = 64;     // members that one wave ranks
-constexpr int WHOLE = 65536;  // rows up to here are one workgroup's
+// Rows up to here are one workgroup's
+constexpr int WHOLE = 65536, WHOLE_16 = 262144;
 
 struct ChunkMax {
   float hi, lo;  // largest; smallest that is not -inf
@@ -97,6 +98,26 @@ __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
   }
   const int tail = first + vecs * VEC + tid;
   if (tail < end) f(tail, as_f32(row[tail]));
+}
+
+// Running sums over the wave's lanes, by DPP: not through LDS.
+__device__ __forceinline__ u64 wave_run_up(u64 v) {
+#define LPX_ADD_FROM(ctrl, rows)                                                   \
+  {                                                                                \
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(                     \
+        0, (int)(unsigned)v, ctrl, rows, 0xf, false);                              \
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(                     \
+        0, (int)(unsigned)(v >> 32), ctrl, rows, 0xf, false);                      \
+    v += (u64)hi << 32 | lo;                                                       \
+  }
+  LPX_ADD_FROM(0x111, 0xf)  // row_shr 1, 2, 4, 8: within 16 lanes
+  LPX_ADD_FROM(0x112, 0xf)
+  LPX_ADD_FROM(0x114, 0xf)
+  LPX_ADD_FROM(0x118, 0xf)
+  LPX_ADD_FROM(0x142, 0xa)  // row_bcast 15 and 31: what stands before them
+  LPX_ADD_FROM(0x143, 0xc)
+#undef LPX_ADD_FROM
+  return v;
 }
 
 // ---- a row's weights and bins --------------------------------------------
@@ -207,6 +228,25 @@ __device__ __forceinline__ u64 weight(const RowScale& r, float x) {
   return (u64)__builtin_bit_cast(long long, w) & 0xfffffffffffffull;
 }
 
+// The least weight that min-p keeps.
+__device__ __forceinline__ u64 least_weight(const SampleArgs& a, int row,
+                                            const RowScale& r) {
+  const double p = fmax(0.0, fmin(param(a.min_p, row), 2.0));
+  return (u64)ceil(p * (double)(1ll << (int)r.shift));
+}
+
+// What a running mass has to reach to hold a share of another; what it has to
+// reach to exceed u times that.
+__device__ __forceinline__ u64 share_of(double part, u64 of) {
+  const double s = ceil(part * (double)of);
+  return s >= (double)of ? of : s > 1 ? (u64)s : (u64)1;
+}
+
+__device__ __forceinline__ u64 draw_border(double u, u64 of) {
+  const double s = floor(u * (double)of);
+  return s >= (double)of ? max(of, (u64)1) : s > 0 ? (u64)s + 1 : (u64)1;
+}
+
 // ---- 1: maxima ------------------------------------------------------------
 
 template <typename T>
@@ -235,10 +275,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_max_kernel(SampleArgs a) 
 // Adds [begin, end) of a row to bins in LDS. Counts are only asked for where
 // the row is cut by top-k or top-p.
 template <int THREADS, typename T, typename B>
-__device__ __forceinline__ void add_bins(B& b, const RowScale& r, double min_p,
+__device__ __forceinline__ void add_bins(B& b, const RowScale& r, u64 least,
                                          const T* row, int begin, int end) {
   const bool counted = r.by_k || r.by_p;
-  const u64 least = (u64)ceil(fmax(0.0, fmin(min_p, 2.0)) * (double)(1ll << (int)r.shift));
   u64 minp = 0;
   scan<THREADS, 2>(row, begin, end, [&](int, float x) {
     const int bin = bin_of(r, x);
@@ -264,7 +303,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a)
   b.count[threadIdx.x] = 0;
   if (threadIdx.x == 0) b.minp = 0;
   __syncthreads();
-  add_bins<CHUNK_THREADS>(b, r, param(a.min_p, row),
+  add_bins<CHUNK_THREADS>(b, r, least_weight(a, row, r),
                           static_cast<const T*>(a.logits) + row * a.stride, begin, end);
   __syncthreads();
   ChunkBins& out = a.bins[blockIdx.x];
@@ -319,17 +358,8 @@ __device__ __forceinline__ void run_up(ChunkBins& b, RowShared& sh) {
   u64 m = 0;
   unsigned c = 0;
   if (t < BINS) {
-    m = b.mass[t];
-    c = b.count[t];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const u64 mm = __shfl_up(m, d, 64);
-      const unsigned cc = __shfl_up(c, d, 64);
-      if (lane >= d) {
-        m += mm;
-        c += cc;
-      }
-    }
+    m = wave_run_up(b.mass[t]);
+    c = (unsigned)wave_run_up((u64)b.count[t]);
     if (lane == 63) {
       sh.wave_mass[t >> 6] = m;
       sh.wave_count[t >> 6] = c;
@@ -515,11 +545,6 @@ __device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
   const unsigned all = sh.row.count[BINS - 1];
   RowPick<T> pick{a, static_cast<const T*>(a.logits) + row * a.stride, r, sh};
 
-  // what a share of a mass has to reach
-  auto share = [](double part, u64 of) {
-    const double s = ceil(part * (double)of);
-    return s >= (double)of ? of : s > 1 ? (u64)s : (u64)1;
-  };
   u64 kept = total;
   const double k = param(a.top_k, row);
   if (r.by_k && k < (double)all) {
@@ -534,17 +559,14 @@ __device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
     }
   }
   if (r.by_p) {
-    const u64 border = share(param(a.top_p, row), kept);
+    const u64 border = share_of(param(a.top_p, row), kept);
     const int bin = bin_at(sh.row, false, border, sh);
     if (!pick.listed(bin) && sh.row.count[bin] <= LIST) pick.collect(0, bin);
     pick.resolve(false, border);
     kept = sh.mass;
   }
   kept = min(kept, sh.row.minp);
-  const double at = floor(param(a.u, row) * (double)kept);
-  pick.resolve(false, at >= (double)kept ? max(kept, (u64)1)
-                      : at > 0           ? (u64)at + 1
-                                         : (u64)1);
+  pick.resolve(false, draw_border(param(a.u, row), kept));
   return sh.at;
 }
 
@@ -579,12 +601,10 @@ __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   if (t == 0) a.token[row] = token;
 }
 
-// All of it in one workgroup, for rows that it reads faster than three
-// kernels follow one another.
+// All of a row in one workgroup.
 template <typename T>
-__global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
-  __shared__ RowShared sh;
-  const int row = (int)blockIdx.x, t = (int)threadIdx.x;
+__device__ __forceinline__ void whole_row(const SampleArgs& a, int row, RowShared& sh) {
+  const int t = (int)threadIdx.x;
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   Extent e;
   scan<ROW_THREADS, 4>(x, 0, a.vocab, [&](int i, float v) {
@@ -604,7 +624,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
     if (t == 0) a.token[row] = r.at;
     return;
   }
-  add_bins<ROW_THREADS>(sh.row, r, param(a.min_p, row), x, 0, a.vocab);
+  add_bins<ROW_THREADS>(sh.row, r, least_weight(a, row, r), x, 0, a.vocab);
   __syncthreads();
   run_up(sh.row, sh);
   const int token = pick_token<T>(a, row, r, sh);
@@ -612,17 +632,394 @@ __global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
 }
 
 template <typename T>
+__global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
+  __shared__ RowShared sh;
+  whole_row<T>(a, (int)blockIdx.x, sh);
+}
+
+// ---- 16-bit rows ----------------------------------------------------------
+// There are 65536 logits of 16 bits, so a row is the count of each: one LDS
+// atomic a logit, and an exp for each of the few thousand values that occur.
+// The borders are then looked up among the values, and where equal logits
+// stand on one, the row is read once more for the index of the one meant.
+//
+// A value's place is its rank from the top: positive ones 0x7fff - bits,
+// negative ones their bits. Ranks below that of +inf are NaN, those from
+// that of -inf on are -inf and NaN.
+
+constexpr int GROUPS = 1024;  // of 64 neighbouring ranks
+
+template <typename T> struct Ranks;
+template <> struct Ranks<__bf16> {
+  static constexpr unsigned INF = 0x7fff - 0x7f80, NONE = 0xff80;
+  static __device__ __forceinline__ float value(unsigned bits) {
+    return __uint_as_float(bits << 16);
+  }
+};
+template <> struct Ranks<_Float16> {
+  static constexpr unsigned INF = 0x7fff - 0x7c00, NONE = 0xfc00;
+  static __device__ __forceinline__ float value(unsigned bits) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+  }
+};
+
+// Bits to rank and back; two values at once.
+__device__ __forceinline__ unsigned ranks_of(unsigned two) {
+  const unsigned positive = ~two & 0x80008000u;
+  return two ^ (positive - (positive >> 15));
+}
+
+struct TableShared {
+  // Rank r's count is in half r >> 15 of word r & 0x7fff. A count of 65536
+  // and more runs over; the counts' sum then falls short of the row's length.
+  unsigned count[32768];
+  u64 mass[GROUPS];        // of 64 ranks; running sums later
+  unsigned members[GROUPS];  // counted for top-k; later for 512 logits each
+  u64 wave_sum[ROW_THREADS / 64], wave_sum2[ROW_THREADS / 64];
+  unsigned first;          // the highest logit's rank
+  unsigned logits;
+  u64 minp;
+  int group;
+  unsigned rank, copy;     // a border's answer: its value, which of equal ones
+  u64 kept;                // and the running mass with it
+  int token;
+};
+
+// f(index of the first, 8 values) / g(index, value) for a row's 16-bit words.
+template <int AHEAD, typename F, typename G>
+__device__ __forceinline__ void scan_words(const unsigned short* row, int n,
+                                           F f, G g) {
+  const int t = (int)threadIdx.x;
+  const int off = (int)(((uintptr_t)row & 15) / 2);
+  const int head = min(off ? 8 - off : 0, n);
+  if (t < head) g(t, (unsigned)row[t]);
+  const int vecs = (n - head) / 8;
+  const i32x4* body = reinterpret_cast<const i32x4*>(row + head);
+  for (int i = t; i < vecs; i += AHEAD * ROW_THREADS) {
+    i32x4 v[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (i + a * ROW_THREADS < vecs) v[a] = body[i + a * ROW_THREADS];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a)
+      if (i + a * ROW_THREADS < vecs) f(head + (i + a * ROW_THREADS) * 8, v[a]);
+  }
+  const int tail = head + vecs * 8 + t;
+  if (tail < n) g(tail, (unsigned)row[tail]);
+}
+
+template <typename T>
+__device__ __forceinline__ float logit_at(unsigned rank) {
+  return Ranks<T>::value((rank >> 15 ? rank : 0x7fffu - rank) & 0xffffu);
+}
+
+__device__ __forceinline__ unsigned count_at(const TableShared& sh, unsigned rank) {
+  return (sh.count[rank & 0x7fff] >> (rank >> 15 ? 16 : 0)) & 0xffffu;
+}
+
+// The value at which the running count (mass) reaches `border`, which of its
+// copies does, and the running mass with that.
+template <typename T>
+__device__ __forceinline__ void find_border(TableShared& sh, const RowScale& r,
+                                            bool by_count, u64 border) {
+  const int t = (int)threadIdx.x;
+  {
+    const u64 now = by_count ? sh.members[t] : sh.mass[t];
+    const u64 before = t == 0 ? 0 : by_count ? sh.members[t - 1] : sh.mass[t - 1];
+    if (now >= border && before < border) sh.group = t;
+  }
+  __syncthreads();
+  if (t < 64) {
+    const int group = sh.group;
+    const unsigned rank = (unsigned)group * 64 + t;
+    const bool some = rank >= Ranks<T>::INF && rank < Ranks<T>::NONE;
+    const u64 n = some ? count_at(sh, rank) : 0;
+    const u64 w = n ? weight(r, logit_at<T>(rank)) : 0;
+    // before this value
+    const u64 mass = (group ? sh.mass[group - 1] : 0) + wave_run_up(n * w) - n * w;
+    const u64 members =
+        by_count ? (group ? sh.members[group - 1] : 0) + wave_run_up(n) - n : 0;
+    const u64 was = by_count ? members : mass, each = by_count ? 1 : w;
+    if (was < border && was + n * each >= border) {
+      // how many copies reach it: border - was of `each`, rounded up
+      u64 need = border - was;
+      if (!by_count) {
+        u64 q = (u64)((double)need / (double)w);
+        while (q * w < need) ++q;
+        while (q > 1 && (q - 1) * w >= need) --q;
+        need = q;
+      }
+      sh.rank = rank;
+      sh.copy = (unsigned)need - 1;
+      sh.kept = mass + need * w;
+    }
+  }
+  __syncthreads();
+}
+
+// Running sums over the workgroup's threads.
+__device__ __forceinline__ u64 block_run_up(u64 v, u64* waves) {
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+  v = wave_run_up(v);
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  const u64 up = wave_run_up(lane < ROW_THREADS / 64 ? waves[lane] : 0);
+  const u64 before = __shfl(up, max(wave - 1, 0), 64);
+  return wave ? v + before : v;
+}
+
+// The index of copy number `copy` of a value: the copies in every 512 logits
+// are counted, and those that hold the one meant looked at again.
+__device__ __forceinline__ int index_of(TableShared& sh, const unsigned short* row,
+                                        int n, unsigned rank, unsigned copy) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const int t = (int)threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  constexpr int WAVES = ROW_THREADS / 64;
+  const unsigned bits = rank >> 15 ? rank : 0x7fffu - rank;
+  const unsigned both = bits << 16 | bits;
+  const unsigned keep = bits ? 0xffffffffu : 0x7fff7fffu;  // -0 is 0
+  auto load = [&](int at) {
+    i32x4 v;
+    if (at + 8 <= n) {
+      __builtin_memcpy(&v, row + at, 16);
+    } else {  // what is not there is not it
+      unsigned short w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        w[j] = at + j < n ? row[at + j] : (unsigned short)(bits ^ 0x4000u);
+      __builtin_memcpy(&v, w, 16);
+    }
+    return v;
+  };
+  // 0 for a logit that is it, otherwise 1
+  auto differ = [&](int v) {
+    const u16x2 d = __builtin_bit_cast(u16x2, ((unsigned)v & keep) ^ both);
+    return __builtin_elementwise_min(d, u16x2{1, 1});
+  };
+  auto copies = [&](i32x4 v) {
+    const u16x2 d = differ(v[0]) + differ(v[1]) + differ(v[2]) + differ(v[3]);
+    return 8u - d[0] - d[1];
+  };
+  sh.members[t] = 0;
+  __syncthreads();
+  const int blocks = (n + 511) / 512;  // GROUPS at most
+  for (int b = wave; b < blocks; b += 4 * WAVES) {
+    i32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (b + j * WAVES < blocks) v[j] = load((b + j * WAVES) * 512 + lane * 8);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (b + j * WAVES >= blocks) break;
+      const unsigned have = copies(v[j]);
+      if (__ballot(have != 0)) {
+        const u64 all = wave_run_up(have);
+        if (lane == 63) sh.members[b + j * WAVES] = (unsigned)all;
+      }
+    }
+  }
+  __syncthreads();
+  const unsigned here = sh.members[t];
+  const unsigned through = (unsigned)block_run_up(here, sh.wave_sum);
+  if (through - here <= copy && copy < through) {
+    sh.group = t;
+    sh.copy = copy - (through - here);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    const int at = sh.group * 512 + lane * 8;
+    const i32x4 v = load(at);
+    const unsigned have = copies(v), up = (unsigned)wave_run_up(have);
+    unsigned left = sh.copy - (up - have);
+    if (up - have <= sh.copy && sh.copy < up) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const u16x2 d = differ(v[j / 2]);
+        if (!d[j % 2] && left-- == 0) sh.token = at + j;
+      }
+    }
+  }
+  __syncthreads();
+  return sh.token;
+}
+
+template <typename T>
+__global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
+  __shared__ union Shared {
+    TableShared table;
+    RowShared row;
+    __device__ Shared() {}
+  } shared;
+  TableShared& sh = shared.table;
+  const int row = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
+  const unsigned short* x = static_cast<const unsigned short*>(a.logits) + row * a.stride;
+  const bool greedy = !(param(a.temperature, row) > 0);
+
+  {
+    const i32x4 zero = {0, 0, 0, 0};
+    i32x4* words = reinterpret_cast<i32x4*>(sh.count);
+    if (!greedy)
+      for (int i = t; i < 8192; i += ROW_THREADS) words[i] = zero;
+    sh.mass[t] = 0;
+    sh.members[t] = 0;
+    if (t == 0) {
+      sh.first = 0xffffu;
+      sh.logits = 0;
+      sh.minp = 0;
+      sh.group = 0;
+      sh.rank = 0;
+      sh.copy = 0;
+      sh.kept = 0;
+      sh.token = -1;
+    }
+  }
+  __syncthreads();
+
+  // Counts, and the highest: of ranks from +inf's on, of which NaN's are not.
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 lows = {0xffff, 0xffff};
+  auto highest = [&](unsigned two) {
+    const u16x2 above = __builtin_bit_cast(u16x2, two) -
+                        u16x2{(unsigned short)Ranks<T>::INF, (unsigned short)Ranks<T>::INF};
+    lows = __builtin_elementwise_min(lows, above);
+  };
+  auto one = [&](unsigned rank) {
+    if (!greedy) atomicAdd(&sh.count[rank & 0x7fff], 1u << (rank >> 15 << 4));
+  };
+  scan_words<4>(
+      x, a.vocab,
+      [&](int, i32x4 v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned two = ranks_of((unsigned)v[j]);
+          highest(two);
+          one(two & 0xffffu);
+          one(two >> 16);
+        }
+      },
+      [&](int, unsigned bits) {
+        const unsigned two = ranks_of(bits << 16 | bits);
+        highest(two);
+        one(two & 0xffffu);
+      });
+  unsigned low = min((unsigned)lows[0], (unsigned)lows[1]);
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) low = min(low, (unsigned)__shfl_xor(low, m, 64));
+  if (lane == 0) atomicMin(&sh.first, low);
+  __syncthreads();
+  unsigned first = sh.first + Ranks<T>::INF;
+  if (first >= Ranks<T>::NONE) {  // nothing over -inf
+    if (t == 0) a.token[row] = -1;
+    return;
+  }
+  if (first == 0x8000u) first = 0x7fffu;
+  if (greedy) {
+    const int token = index_of(sh, x, a.vocab, first, 0);
+    if (t == 0) a.token[row] = token;
+    return;
+  }
+  if (t == 0) {  // -0 is 0
+    const unsigned both = sh.count[0x7fff] & 0xffffu, minus = sh.count[0] >> 16;
+    if (both + minus < 65536u) {
+      sh.count[0x7fff] += minus;
+      sh.count[0] &= 0xffffu;
+    } else {
+      sh.count[0x7fff] &= 0xffff0000u;  // too many: the sum will say so
+    }
+  }
+  __syncthreads();
+
+  Extent e;
+  e.hi = e.lo = logit_at<T>(first);
+  e.at = 0;
+  const RowScale r = row_scale(a, row, e);
+  const u64 least = least_weight(a, row, r);
+  // Sums of groups of 64 ranks. Most words hold nothing: a wave looks at 256
+  // of them at once, and at the groups of those that do one by one.
+  u64 minp = 0;
+  unsigned all = 0;
+  for (int b = wave; b < 128; b += ROW_THREADS / 64) {
+    const i32x4 v = *reinterpret_cast<const i32x4*>(sh.count + b * 256 + lane * 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) all += ((unsigned)v[j] & 0xffffu) + ((unsigned)v[j] >> 16);
+    if (!__ballot((v[0] | v[1] | v[2] | v[3]) != 0)) continue;
+    unsigned two[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two[j] = sh.count[b * 256 + j * 64 + lane];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int group = b * 4 + (j & 3) + (j >> 2) * (GROUPS / 2);
+      const unsigned rank = (unsigned)group * 64 + lane;
+      unsigned n = j >> 2 ? two[j & 3] >> 16 : two[j & 3] & 0xffffu;
+      if (rank < Ranks<T>::INF || rank >= Ranks<T>::NONE) n = 0;
+      if (!__ballot(n != 0)) continue;
+      const u64 w = weight(r, logit_at<T>(rank));
+      u64 mass = n * w;
+      if (w >= least) minp += mass;
+      mass = wave_run_up(mass);
+      unsigned members = 0;
+      if (r.by_k) members = (unsigned)wave_run_up((u64)n);
+      if (lane == 63) {
+        sh.mass[group] = mass;
+        sh.members[group] = members;
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) {
+    all += __shfl_xor(all, m, 64);
+    minp += __shfl_xor(minp, m, 64);
+  }
+  if (lane == 0) {
+    atomicAdd(&sh.logits, all);
+    atomicAdd(&sh.minp, minp);
+  }
+  __syncthreads();
+  if (sh.logits != (unsigned)a.vocab) {  // uniform: the row has to be kept whole
+    __syncthreads();
+    whole_row<T>(a, row, shared.row);
+    return;
+  }
+  // Running sums; thread t has group t
+  {
+    const u64 m = block_run_up(sh.mass[t], sh.wave_sum);
+    const u64 n = r.by_k ? block_run_up(sh.members[t], sh.wave_sum2) : 0;
+    sh.mass[t] = m;
+    sh.members[t] = (unsigned)n;
+  }
+  __syncthreads();
+
+  u64 kept = sh.mass[GROUPS - 1];
+  const double k = param(a.top_k, row);
+  if (r.by_k && k < (double)sh.members[GROUPS - 1]) {
+    find_border<T>(sh, r, true, (u64)k);
+    kept = sh.kept;
+  }
+  if (r.by_p) {
+    find_border<T>(sh, r, false, share_of(param(a.top_p, row), kept));
+    kept = sh.kept;
+  }
+  kept = min(kept, sh.minp);
+  find_border<T>(sh, r, false, draw_border(param(a.u, row), kept));
+  const int token = index_of(sh, x, a.vocab, sh.rank, sh.copy);
+  if (t == 0) a.token[row] = token;
+}
+
+template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
+  const dim3 rows((unsigned)a.rows), threads(ROW_THREADS);
   if (a.chunks == 0) {
-    row_whole_kernel<T>
-        <<<dim3((unsigned)a.rows), dim3(ROW_THREADS), 0, stream>>>(a);
+    if constexpr (sizeof(T) == 2)
+      row_table_kernel<T><<<rows, threads, 0, stream>>>(a);
+    else
+      row_whole_kernel<T><<<rows, threads, 0, stream>>>(a);
     return hipGetLastError();
   }
   const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
   chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
   chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
-  row_pick_kernel<T>
-      <<<dim3((unsigned)a.rows), dim3(ROW_THREADS), 0, stream>>>(a);
+  row_pick_kernel<T><<<rows, threads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -631,12 +1028,12 @@ struct Plan {
   size_t maxima_bytes, bytes;
 };
 
-Plan plan_of(int rows, int vocab) {
+Plan plan_of(int rows, int vocab, bool half) {
   // At least 4096 logits a chunk; more where there are chunks enough for the
   // chip without that, so that fewer histograms are written.
   const long want = ((long)rows * vocab + 2047) / 2048;
   Plan p{};
-  if (vocab <= WHOLE) return p;
+  if (vocab <= (half ? WHOLE_16 : WHOLE)) return p;
   p.chunk = (int)(want < 4096 ? 4096 : (want + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
@@ -646,8 +1043,8 @@ Plan plan_of(int rows, int vocab) {
 
 }  // namespace
 
-size_t sample_workspace(int rows, int vocab) {
-  return rows > 0 && vocab > 0 ? plan_of(rows, vocab).bytes : 0;
+size_t sample_workspace(ActType t, int rows, int vocab) {
+  return rows > 0 && vocab > 0 ? plan_of(rows, vocab, t != ActType::f32).bytes : 0;
 }
 
 hipError_t sample(ActType t, const void* logits, long stride, int rows,
@@ -656,7 +1053,7 @@ hipError_t sample(ActType t, const void* logits, long stride, int rows,
                   void* workspace, int64_t* token, hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
   if (vocab <= 0) return hipErrorInvalidValue;
-  const Plan p = plan_of(rows, vocab);
+  const Plan p = plan_of(rows, vocab, t != ActType::f32);
   if ((int64_t)rows * p.chunks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
   int shift = 45;  // sums of `vocab` weights stay below 2^62
   while (vocab > (int64_t(1) << (62 - shift))) --shift;

@@ -699,3 +699,49 @@ def test_sample_refuses():
             (lambda: ops.sample(x, u), "on the ROCm device")):
         with pytest.raises(RuntimeError, match=why):
             bad()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [300, 65535, 65537, 70000, 140001])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=30), dict(top_k=5000), dict(top_p=0.4),
+                                      dict(top_k=4999, top_p=0.8), dict(min_p=0.5),
+                                      dict(temperature=0.0)])
+def test_sample_ties_of_16_bits(dtype, v, settings):
+    # more equal logits than 16 bits count, on both sides of zero
+    one = torch.full((v,), 1.5)
+    low = torch.full((v,), -3.0)
+    low[v // 2] = -2.0
+    few = (torch.arange(v) * 7919 % 5).float() - 4.0
+    zero = torch.where(torch.arange(v) % 2 == 0, 0.0, -0.0)
+    x = torch.stack([one, low, few, zero] * 4).to(dtype).to(DEV)
+    u = torch.linspace(0.013, 0.987, 16).to(DEV)
+    got = ops.sample(x, u, **settings)
+    assert _same_tokens(got, x, u, **settings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=50), dict(top_p=0.9), dict(temperature=0.0),
+                                      dict(temperature=1e-3), dict(temperature=1e4, top_p=0.3)])
+def test_sample_masked_rows_of_16_bits(dtype, settings):
+    v = 20001
+    x = _randn((10, v), 65, scale=3.0).to(dtype)
+    inf, least = float("inf"), torch.finfo(dtype).min
+    x[0] = -inf
+    x[1] = -inf
+    x[1, 777] = -5.0
+    x[2, :19000] = least
+    x[3, ::2] = float("nan")
+    x[3, 1::4] = -torch.tensor(float("nan"))
+    x[4, 11] = x[4, 19999] = inf
+    x[5] = least
+    x[6, 5], x[6, 6] = torch.finfo(dtype).max, least
+    x[7] = float("nan")
+    x[8, :] = -inf
+    x[8, 100:400] = torch.randn(300, generator=_gen(66)).to(dtype).to(DEV)
+    x[9] = x[9] * 2.0 ** -14
+    u = torch.linspace(0.05, 0.95, 10).to(DEV)
+    got = ops.sample(x, u, **settings)
+    assert _same_tokens(got, x, u, **settings)
+    assert got[0] == -1 and got[7] == -1 and got[1] == 777
