@@ -8,14 +8,20 @@
 //
 // All three filters and the draw ask the same thing of the sorted row: where
 // does a running count or a running weight pass a border. Nothing is sorted
-// for that. Weights are 64-bit integers (w_i * 2^45, rounded), so their sums
-// do not depend on the order of adding and a histogram's totals agree with
-// its members' to the last bit: 256 bins, linear in x below the maximum, tell
-// the bin that holds a border, and only that bin's members are looked at.
+// for that. Weights are 64-bit integers (w_i * 2^45, rounded), so that their
+// sums do not depend on the order of adding: a border in a flat row of 10^5
+// logits is decided by the 10th digit of a sum.
 //
-// Three launches: the maxima of chunks of rows; the chunks' histograms (one
-// exp a logit, in 64 bits: a border in a flat row of 10^5 logits is decided by
-// the 10th digit of a sum); one workgroup a row that finds the borders.
+// 16-bit rows: one workgroup a row counts each of the 65536 values in LDS and
+// looks the borders up among them; the exps are as many as the values that
+// occur. 256 x 131072 bf16: 34 us (the LDS atomics of the counting take 10,
+// reading the row a second time for the index 8); 1 x 32000: 15 us.
+//
+// f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
+// bin that holds a border, and only that bin's members are looked at. An exp
+// a logit in 64 bits, 33 instructions, is what that takes. Short rows in one
+// workgroup each; long ones as chunks (maxima, then histograms) and one
+// workgroup a row for the borders: 24 x 50001 28 us, 256 x 131072 98 us.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -29,10 +35,13 @@ typedef unsigned long long u64;
 constexpr int BINS = 256;
 constexpr int CHUNK_THREADS = 256;
 constexpr int ROW_THREADS = 1024;
-constexpr int LIST = 4096;  // members of bins kept in LDS
+constexpr int LIST = 512;   // members of bins that a wave keeps in LDS
 constexpr int FEW = 64;     // members that one wave ranks
 // Rows up to here are one workgroup's
-constexpr int WHOLE = 65536, WHOLE_16 = 262144;
+// (16 bits: those whose counts of 512 logits fit the table). f32 by measured
+// time: one row of 16000 takes 16 us so and 19 as chunks, of 32000 24 and 22;
+// 256 rows of 32000 30 and 40, of 64000 49 and 58.
+constexpr int WHOLE = 24576, WHOLE_MANY = 65536, MANY = 96, WHOLE_16 = 262144;
 
 struct ChunkMax {
   float hi, lo;  // largest; smallest that is not -inf
@@ -326,19 +335,38 @@ __device__ __forceinline__ float logit_of(u64 o) {
   return __uint_as_float(up ^ ((up >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
+// The lowest logit in bin `bin` or above, which is where the bin begins. The
+// wave looks at 64 of f32's values at a time, in the order of their bits.
+__device__ __forceinline__ float bin_begin(const RowScale& r, int bin) {
+  const auto up = [](float x) { return ~(unsigned)(order_of(x, 0) >> 32); };
+  const unsigned most = up(r.hi), least = up(-3.402823466e38f);
+  unsigned at = 0;
+#pragma unroll
+  for (int shift = 26; shift >= -4; shift -= 6) {
+    const int s = max(shift, 0);
+    const unsigned lane = threadIdx.x & 63;
+    const unsigned last = at + (lane << s) + ((1u << s) - 1);
+    const bool over = last < at;  // past the highest bits
+    const unsigned key = over ? most : max(min(last, most), least);
+    const u64 in = __ballot(bin_of(r, logit_of((u64)~key << 32)) <= bin);
+    at += (unsigned)__builtin_ctzll(in) << s;
+  }
+  return logit_of((u64)~max(min(at, most), least) << 32);
+}
+
 struct Member {
   u64 order, weight;
 };
 
 struct RowShared {
   ChunkBins row, sub;  // running sums, bin by bin
-  u64 list[LIST];
+  u64 list[ROW_THREADS / 64][LIST];
+  int listed[ROW_THREADS / 64];
   Member few[FEW];
   ChunkMax extent[ROW_THREADS / 64];
   u64 wave_mass[BINS / 64];
   unsigned wave_count[BINS / 64];
   u64 lo, hi;
-  unsigned n;
   int bin, found;
   u64 mass;  // a border's answer
   int at;
@@ -400,7 +428,8 @@ struct RowPick {
   const T* row;
   const RowScale r;
   RowShared& sh;
-  int first = 0, last = -1;  // the bins whose members are in the list
+  int first = 0, last = -1;  // the bins whose members are in the lists
+  unsigned found = 0;        // and how many they are
 
   __device__ __forceinline__ bool listed(int bin) const {
     return first <= bin && bin <= last;
@@ -410,9 +439,9 @@ struct RowPick {
   template <typename F>
   __device__ __forceinline__ void members(int bin, u64 lo, u64 hi, F f) {
     if (listed(bin)) {
-      const int n = (int)min(sh.n, (unsigned)LIST);
-      for (int i = (int)threadIdx.x; i < n; i += ROW_THREADS) {
-        const u64 o = sh.list[i];
+      const int wave = (int)threadIdx.x >> 6, n = sh.listed[wave];
+      for (int i = (int)threadIdx.x & 63; i < n; i += 64) {
+        const u64 o = sh.list[wave][i];
         const float x = logit_of(o);
         if (bin_of(r, x) == bin && lo <= o && o <= hi) f(o, x);
       }
@@ -425,22 +454,65 @@ struct RowPick {
     }
   }
 
-  // Lists the members of bins [from, to], unless they are more than LIST.
+  // Lists the members of bins [from, to], unless a wave's are too many.
   // Returns how many they are.
   __device__ __forceinline__ unsigned collect(int from, int to) {
-    if (threadIdx.x == 0) sh.n = 0;
-    __syncthreads();
-    scan<ROW_THREADS, 4>(row, 0, a.vocab, [&](int i, float x) {
-      const int bin = bin_of(r, x);
-      if (from <= bin && bin <= to && real(x)) {
-        const unsigned n = atomicAdd(&sh.n, 1u);
-        if (n < LIST) sh.list[n] = order_of(x, i);
+    constexpr int VEC = 16 / sizeof(T), AHEAD = 4;
+    typedef T V __attribute__((ext_vector_type(VEC)));
+    // the bins as an interval, so that a logit takes two comparisons
+    const float low = bin_begin(r, to);
+    const float above = bin_of(r, r.hi) < from ? bin_begin(r, from - 1) : __builtin_inff();
+    const bool top = above == __builtin_inff();  // which then belongs to it
+    const int lane = (int)threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    // Each wave has a list of its own and knows its length: no atomic, whose
+    // answer would have to be waited for. All lanes come here together.
+    int have = 0;
+    auto add = [&](bool there, int i, float x) {
+      const bool in = there && low <= x && (x < above || top);
+      const u64 who = __ballot(in);
+      if (!who) return;
+      const int at = have + (int)__builtin_amdgcn_mbcnt_hi(
+                                (unsigned)(who >> 32),
+                                __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
+      if (in && at < LIST) sh.list[wave][at] = order_of(x, i);
+      have += __popcll(who);
+    };
+    const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
+    const int head = min(off ? VEC - off : 0, a.vocab);
+    const int vecs = (a.vocab - head) / VEC;
+    const V* body = reinterpret_cast<const V*>(row + head);
+    if (wave == 0) {
+      const int tail = head + vecs * VEC + lane;
+      add(lane < head, lane, lane < head ? as_f32(row[lane]) : 0.f);
+      add(tail < a.vocab, tail, tail < a.vocab ? as_f32(row[tail]) : 0.f);
+    }
+    for (int v0 = wave * 64; v0 < vecs; v0 += AHEAD * ROW_THREADS) {
+      V v[AHEAD];
+#pragma unroll
+      for (int l = 0; l < AHEAD; ++l)
+        v[l] = body[min(v0 + l * ROW_THREADS + lane, vecs - 1)];
+#pragma unroll
+      for (int l = 0; l < AHEAD; ++l) {
+        const int at = v0 + l * ROW_THREADS + lane;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          add(at < vecs, head + at * VEC + j, as_f32(v[l][j]));
       }
-    });
+    }
+    if (lane == 0) sh.listed[wave] = have;
     __syncthreads();
+    unsigned all = 0;
+    bool fits = true;
+    for (int w = 0; w < ROW_THREADS / 64; ++w) {
+      const int n = sh.listed[w];
+      all += n;
+      fits &= n <= LIST;
+    }
     first = from;
-    last = sh.n <= LIST ? to : from - 1;
-    return sh.n;
+    last = fits ? to : from - 1;
+    found = all;
+    return all;
   }
 
   // The member of the row at which the running count (mass) reaches `border`:
@@ -453,7 +525,7 @@ struct RowPick {
     unsigned n;
     if (listed(bin)) {
       const unsigned members = sh.row.count[bin] - base;
-      n = first == last ? sh.n : members;
+      n = first == last ? found : members;
     } else {
       n = collect(bin, bin);
     }
@@ -550,7 +622,7 @@ __device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
   if (r.by_k && k < (double)all) {
     const unsigned want = (unsigned)k;
     const int bin = bin_at(sh.row, true, want, sh);
-    if (sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    if (sh.row.count[bin] <= LIST * 8) pick.collect(0, bin);
     if (sh.row.count[bin] == want) {
       kept = sh.row.mass[bin];
     } else {
@@ -561,7 +633,7 @@ __device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
   if (r.by_p) {
     const u64 border = share_of(param(a.top_p, row), kept);
     const int bin = bin_at(sh.row, false, border, sh);
-    if (!pick.listed(bin) && sh.row.count[bin] <= LIST) pick.collect(0, bin);
+    if (!pick.listed(bin) && sh.row.count[bin] <= LIST * 8) pick.collect(0, bin);
     pick.resolve(false, border);
     kept = sh.mass;
   }
@@ -574,27 +646,27 @@ template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   __shared__ RowShared sh;
   const int row = (int)blockIdx.x, t = (int)threadIdx.x;
+  // thread t sums bin t % BINS over a quarter of the chunks
+  const ChunkBins* c = a.bins + (long)row * a.chunks;
+  const int bin = t % BINS;
+  u64 m = 0, minp = 0;
+  unsigned n = 0;
+#pragma unroll 4
+  for (int i = t / BINS; i < a.chunks; i += ROW_THREADS / BINS) {
+    m += c[i].mass[bin];
+    n += c[i].count[bin];
+    if (bin == 0) minp += c[i].minp;
+  }
+  clear(sh.row);
   const RowScale r = row_scale(a, row, row_extent(a, row));
   if (r.greedy) {
     if (t == 0) a.token[row] = r.at;
     return;
   }
-  clear(sh.row);
   __syncthreads();
-  {
-    const ChunkBins* c = a.bins + (long)row * a.chunks;
-    u64 m = 0;
-    unsigned n = 0;
-    const int bin = t % BINS;
-    for (int i = t / BINS; i < a.chunks; i += ROW_THREADS / BINS) {
-      m += c[i].mass[bin];
-      n += c[i].count[bin];
-    }
-    atomicAdd(&sh.row.mass[bin], m);
-    atomicAdd(&sh.row.count[bin], n);
-    for (int i = t; i < a.chunks; i += ROW_THREADS)
-      atomicAdd(&sh.row.minp, c[i].minp);
-  }
+  atomicAdd(&sh.row.mass[bin], m);
+  atomicAdd(&sh.row.count[bin], n);
+  if (bin == 0) atomicAdd(&sh.row.minp, minp);
   __syncthreads();
   run_up(sh.row, sh);
   const int token = pick_token<T>(a, row, r, sh);
@@ -1033,7 +1105,7 @@ Plan plan_of(int rows, int vocab, bool half) {
   // chip without that, so that fewer histograms are written.
   const long want = ((long)rows * vocab + 2047) / 2048;
   Plan p{};
-  if (vocab <= (half ? WHOLE_16 : WHOLE)) return p;
+  if (vocab <= (half ? WHOLE_16 : rows >= MANY ? WHOLE_MANY : WHOLE)) return p;
   p.chunk = (int)(want < 4096 ? 4096 : (want + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
