@@ -9,10 +9,14 @@
 // The norm is taken of the unrounded f32 sum, y is rounded once, and the sum
 // of squares is held in f32 (at most 64 terms a thread, then a tree).
 //
-// One workgroup a row: the row stays in registers between the two uses of
-// it, so each input is read once and each output written once. A thread owns
-// 8 neighbouring elements a step (16-B loads of 16-bit types), an MX block is
-// four neighbouring lanes, a 128-element scale tile sixteen.
+// The row stays in registers between the two uses of it, so each input is
+// read once and each output written once; memory bounds it. A thread owns 8
+// neighbouring elements (16-B loads of 16-bit types), an MX block is four
+// neighbouring lanes, a 128-element scale tile sixteen. One step a thread and
+// as many threads as the row needs: 16384 x 8192 bf16 with residual to MX 204
+// us with 256 threads of four steps each, 174 with 1024 of one, 162 (5.8
+// TB/s) where the stores also pass by the caches; a copy of that size in
+// torch reaches 4.9.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -42,9 +46,11 @@ __device__ __forceinline__ f32x8 load8(const T* p) {
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, f32x8 f) {
+  typedef int words __attribute__((ext_vector_type(sizeof(T) * 2), aligned(sizeof(T))));
   const typename Vec8<T>::type v =
       __builtin_convertvector(f, typename Vec8<T>::type);
-  __builtin_memcpy(p, &v, sizeof(v));
+  __builtin_nontemporal_store(__builtin_bit_cast(words, v),
+                              reinterpret_cast<words*>(p));
 }
 
 // Elements [c, c+8) of a row of K; what lies behind K is 0.
@@ -69,15 +75,13 @@ __device__ __forceinline__ void store_row(T* row, int c, int K, f32x8 v) {
     if (c + j < K) row[c + j] = (T)v[j];
 }
 
-template <int TPR>
 __device__ __forceinline__ float block_sum(float v) {
-  __shared__ float part[TPR / 64];
+  __shared__ float part[16];
   v = lpx_wave_allreduce_sum(v);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0.f;
-#pragma unroll
-  for (int i = 0; i < TPR / 64; ++i) v += part[i];
+  for (unsigned i = 0; i < blockDim.x / 64; ++i) v += part[i];
   return v;
 }
 
@@ -91,7 +95,8 @@ __device__ __forceinline__ unsigned mx_scale_byte(float amax) {
 }
 
 // y[c .. c+8) as MX e4m3. All lanes of the wave come here together; lanes
-// with c >= K bring zeros and store nothing.
+// with c >= K bring zeros and store nothing. A row's lanes are neighbours, 8
+// (K = 64) or a multiple of 16.
 __device__ __forceinline__ void store_mx(unsigned char* __restrict__ qrow,
                                          unsigned char* __restrict__ sc,
                                          int row, int R, int c, int K,
@@ -103,9 +108,10 @@ __device__ __forceinline__ void store_mx(unsigned char* __restrict__ qrow,
   amax = fmaxf(amax, __shfl_xor(amax, 2, 64));
   const unsigned byte = mx_scale_byte(amax);
   const float scale = __uint_as_float(byte << 23);
-  unsigned tile = byte << (8 * ((threadIdx.x >> 2) & 3));
+  unsigned tile = byte << (8 * ((c >> 5) & 3));
   tile |= __shfl_xor(tile, 4, 64);
-  tile |= __shfl_xor(tile, 8, 64);
+  const unsigned more = __shfl_xor(tile, 8, 64);
+  tile |= K > 64 ? more : 0x7f7f0000u;
   if (c >= K) return;
   i32x2 out;
 #pragma unroll
@@ -120,7 +126,8 @@ __device__ __forceinline__ void store_mx(unsigned char* __restrict__ qrow,
   // 64-groups are kept as their quarters [q0 | q2 | q1 | q3]
   const int quarter = (c >> 4) & 3;
   const int slot = ((quarter & 1) << 1) | (quarter >> 1);
-  *reinterpret_cast<i32x2*>(qrow + (c & ~63) + slot * 16 + (c & 8)) = out;
+  __builtin_nontemporal_store(
+      out, reinterpret_cast<i32x2*>(qrow + (c & ~63) + slot * 16 + (c & 8)));
   if ((c & 127) == 0)
     *reinterpret_cast<unsigned*>(sc + ((long)(c >> 7) * R + row) * 4) = tile;
 }
@@ -170,24 +177,38 @@ __device__ __forceinline__ float square_sum(f32x8 h) {
   return s;
 }
 
-// Rows of at most TPR * ITERS * 8 elements, held in registers.
-template <typename T, bool MX, int TPR, int ITERS>
-__global__ __launch_bounds__(TPR) void rmsnorm_kernel(NormArgs a) {
+// Rows of at most 512: `lanes` (a power of two, 8 at least) of a wave each.
+template <typename T, bool MX>
+__global__ __launch_bounds__(256) void rmsnorm_short_kernel(NormArgs a, int lanes) {
+  const int rows = 256 / lanes;
+  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x) * rows +
+                  (int)threadIdx.x / lanes;
+  const int c = row < a.R ? (int)threadIdx.x % lanes * 8 : a.K;
+  f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (c < a.K) h = read_h<T>(a, row, c, true);
+  float s = square_sum(h);
+  for (int m = lanes / 2; m > 0; m >>= 1) s += __shfl_xor(s, m, 64);
+  finish8<T, MX>(a, row, c, h, rsqrtf(s / (float)a.K + a.eps));
+}
+
+// Rows of at most blockDim * STEPS * 8 elements.
+template <typename T, bool MX, int STEPS>
+__global__ __launch_bounds__(1024) void rmsnorm_kernel(NormArgs a) {
   // neighbouring rows on one XCD: their scale bytes share lines of its L2
   const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
-  f32x8 h[ITERS];
+  f32x8 h[STEPS];
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    const int c = (i * TPR + (int)threadIdx.x) * 8;
+  for (int i = 0; i < STEPS; ++i) {
+    const int c = (int)(i * blockDim.x + threadIdx.x) * 8;
     h[i] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
     if (c < a.K) h[i] = read_h<T>(a, row, c, true);
     s += square_sum(h[i]);
   }
-  const float inv = rsqrtf(block_sum<TPR>(s) / (float)a.K + a.eps);
+  const float inv = rsqrtf(block_sum(s) / (float)a.K + a.eps);
 #pragma unroll
-  for (int i = 0; i < ITERS; ++i)
-    finish8<T, MX>(a, row, (i * TPR + (int)threadIdx.x) * 8, h[i], inv);
+  for (int i = 0; i < STEPS; ++i)
+    finish8<T, MX>(a, row, (int)(i * blockDim.x + threadIdx.x) * 8, h[i], inv);
 }
 
 // Longer rows: read a second time (the first pass left them in the caches).
@@ -200,7 +221,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
     const int c = (i * 1024 + (int)threadIdx.x) * 8;
     if (c < a.K) s += square_sum(read_h<T>(a, row, c, true));
   }
-  const float inv = rsqrtf(block_sum<1024>(s) / (float)a.K + a.eps);
+  const float inv = rsqrtf(block_sum(s) / (float)a.K + a.eps);
   for (int i = 0; i < steps; ++i) {
     const int c = (i * 1024 + (int)threadIdx.x) * 8;
     f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -211,17 +232,24 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
 
 template <typename T, bool MX>
 hipError_t launch(const NormArgs& a, hipStream_t stream) {
-  const dim3 grid((unsigned)a.R);
-  if (a.K <= 2048)
-    rmsnorm_kernel<T, MX, 256, 1><<<grid, dim3(256), 0, stream>>>(a);
-  else if (a.K <= 4096)
-    rmsnorm_kernel<T, MX, 256, 2><<<grid, dim3(256), 0, stream>>>(a);
-  else if (a.K <= 8192)
-    rmsnorm_kernel<T, MX, 256, 4><<<grid, dim3(256), 0, stream>>>(a);
-  else if (a.K <= 32768)
-    rmsnorm_kernel<T, MX, 1024, 4><<<grid, dim3(1024), 0, stream>>>(a);
+  const int threads = (a.K + 7) / 8;
+  if (threads <= 64) {
+    int lanes = 8;
+    while (lanes < threads) lanes *= 2;
+    const int rows = 256 / lanes;
+    rmsnorm_short_kernel<T, MX>
+        <<<dim3((unsigned)((a.R + rows - 1) / rows)), dim3(256), 0, stream>>>(a, lanes);
+    return hipGetLastError();
+  }
+  const dim3 grid((unsigned)a.R), block((unsigned)((threads + 63) / 64 * 64)), most(1024);
+  if (threads <= 1024)
+    rmsnorm_kernel<T, MX, 1><<<grid, block, 0, stream>>>(a);
+  else if (threads <= 2048)
+    rmsnorm_kernel<T, MX, 2><<<grid, most, 0, stream>>>(a);
+  else if (threads <= 4096)
+    rmsnorm_kernel<T, MX, 4><<<grid, most, 0, stream>>>(a);
   else
-    rmsnorm_long_kernel<T, MX><<<grid, dim3(1024), 0, stream>>>(a);
+    rmsnorm_long_kernel<T, MX><<<grid, most, 0, stream>>>(a);
   return hipGetLastError();
 }
 

@@ -745,3 +745,27 @@ def test_sample_masked_rows_of_16_bits(dtype, settings):
     got = ops.sample(x, u, **settings)
     assert _same_tokens(got, x, u, **settings)
     assert got[0] == -1 and got[7] == -1 and got[1] == 777
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,k", [(1, 64), (37, 64), (3, 128), (70, 128), (9, 192),
+                                    (5, 256), (33, 320), (131, 512), (3, 576), (2, 16384),
+                                    (2, 16448)])
+def test_rmsnorm_narrow_rows_and_neighbours(rows, k, dtype):
+    # several rows to a wave: each has its own sum and its own scale tile
+    x = _randn((rows, k), 80, dtype) * torch.exp2(
+        torch.arange(rows, device=DEV) % 9 - 4.0).to(dtype).unsqueeze(1)
+    w = _randn((k,), 81, dtype)
+    y = ops.rmsnorm(x, w)
+    assert _near(y, _norm64(x, w, None, 1e-6)[0], _u(dtype) + NORM_REL, dtype)
+    q, sc = ops.rmsnorm_mx(x, w)
+    one = [ops.rmsnorm_mx(x[i:i + 1], w) for i in range(rows)]
+    assert torch.equal(q, torch.cat([o[0] for o in one]))
+    assert torch.equal(sc, torch.cat([o[1] for o in one], dim=1))
+    y64 = _norm64(x, w, None, 1e-6)[0]
+    s = torch.exp2(_mx_rows(sc, k).double() - 127).repeat_interleave(32, dim=1)
+    err = (_mx_values(q, sc) - y64).abs()
+    assert bool((err <= torch.maximum(2.0 ** -4 * y64.abs(), s * 2.0 ** -10)
+                 + 2 * NORM_REL * y64.abs()).all())
+    assert bool((sc.permute(1, 0, 2).flatten(1)[:, k // 32:] == 127).all())
