@@ -6,6 +6,7 @@
 
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
@@ -787,6 +788,11 @@ lpx::ActType act_type(const at::Tensor& t, const char* what) {
   }
 }
 
+// A result's memory, without the dispatcher: for one token a call is host time.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 // Rows of a 2-D view whose last axis is dense; rows may be further apart.
 at::Tensor dense_rows(const at::Tensor& t) {
   const at::Tensor v = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -823,7 +829,7 @@ NormCall norm_call(const at::Tensor& x, const at::Tensor& weight,
   c.w = weight.contiguous();
   if (residual.has_value()) {
     c.r = dense_rows(*residual);
-    c.h = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+    c.h = fresh(x.sizes(), x.scalar_type(), x);
   }
   c.R = (int)c.x.size(0);
   c.K = (int)K;
@@ -834,7 +840,7 @@ std::vector<at::Tensor> rmsnorm(const at::Tensor& x, const at::Tensor& weight,
                                 const std::optional<at::Tensor>& residual, double eps) {
   NormCall c = norm_call(x, weight, residual, eps, "rmsnorm");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-  auto y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  auto y = fresh(x.sizes(), x.scalar_type(), x);
   check_hip(lpx::rmsnorm(c.type, c.x.data_ptr(), c.x.stride(0),
                          c.r.defined() ? c.r.data_ptr() : nullptr,
                          c.r.defined() ? c.r.stride(0) : 0, c.w.data_ptr(),
@@ -851,8 +857,8 @@ std::vector<at::Tensor> rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 64 == 0, "rmsnorm_mx expects x [..., K%64==0]");
   NormCall c = norm_call(x, weight, residual, eps, "rmsnorm_mx");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-  auto q = at::empty({c.R, c.K}, x.options().dtype(at::kByte));
-  auto sc = at::empty({(c.K + 127) / 128, c.R, 4}, x.options().dtype(at::kByte));
+  auto q = fresh({c.R, c.K}, at::kByte, x);
+  auto sc = fresh({(c.K + 127) / 128, c.R, 4}, at::kByte, x);
   check_hip(lpx::rmsnorm_mx(c.type, c.x.data_ptr(), c.x.stride(0),
                             c.r.defined() ? c.r.data_ptr() : nullptr,
                             c.r.defined() ? c.r.stride(0) : 0, c.w.data_ptr(),
@@ -895,9 +901,7 @@ at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor&
   if (rows.stride(0) > (1 << 24)) rows = rows.contiguous();
   auto sizes = x.sizes().vec();
   sizes.back() = N;
-  auto y = at::empty(sizes, x.options()
-                                .dtype(bf16_out ? at::kBFloat16 : at::kFloat)
-                                .memory_format(at::MemoryFormat::Contiguous));
+  auto y = fresh(sizes, bf16_out ? at::kBFloat16 : at::kFloat, x);
   check_hip(lpx::gemv_w4(act_type(x, "gemv_w4"), rows.data_ptr(), rows.stride(0),
                          Bt4.data_ptr<uint8_t>(), sB.data_ptr<uint8_t>(), y.data_ptr(),
                          bf16_out, (int)rows.size(0), (int)N, (int)K, current_stream(x)),
@@ -921,7 +925,7 @@ at::Tensor gemv_mx_w4(const at::Tensor& A, const at::Tensor& sA, const at::Tenso
   TORCH_CHECK(sA.device() == A.device() && Bt4.device() == A.device() &&
               sB.device() == A.device(), "gemv_mx_w4: all tensors must be on one device");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(A.device());
-  auto y = at::empty({M, N}, A.options().dtype(bf16_out ? at::kBFloat16 : at::kFloat));
+  auto y = fresh({M, N}, bf16_out ? at::kBFloat16 : at::kFloat, A);
   check_hip(lpx::gemv_mx_w4(A.data_ptr<uint8_t>(), sA.data_ptr<uint8_t>(),
                             Bt4.data_ptr<uint8_t>(), sB.data_ptr<uint8_t>(), y.data_ptr(),
                             bf16_out, (int)M, (int)N, (int)K, current_stream(A)),
@@ -975,10 +979,9 @@ at::Tensor sample(const at::Tensor& logits, const at::Tensor& u, const Setting& 
   TORCH_CHECK(logits.is_cuda(), "sample: logits must be on the ROCm device (got CPU)");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
   const at::Tensor x = dense_rows(logits);
-  auto token = at::empty(logits.sizes().slice(0, logits.dim() - 1),
-                         logits.options().dtype(at::kLong));
-  auto work = at::empty({(int64_t)lpx::sample_workspace(type, (int)rows, (int)V)},
-                        logits.options().dtype(at::kByte));
+  auto token = fresh(logits.sizes().slice(0, logits.dim() - 1), at::kLong, logits);
+  const auto bytes = (int64_t)lpx::sample_workspace(type, (int)rows, (int)V);
+  const at::Tensor work = bytes ? fresh({bytes}, at::kByte, logits) : token;
   check_hip(lpx::sample(type, x.data_ptr(), x.stride(0), (int)rows, (int)V, t, k, p, q, draw,
                         work.data_ptr(), token.data_ptr<int64_t>(), current_stream(logits)),
             "sample");
