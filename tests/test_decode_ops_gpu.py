@@ -769,3 +769,102 @@ def test_rmsnorm_narrow_rows_and_neighbours(rows, k, dtype):
     assert bool((err <= torch.maximum(2.0 ** -4 * y64.abs(), s * 2.0 ** -10)
                  + 2 * NORM_REL * y64.abs()).all())
     assert bool((sc.permute(1, 0, 2).flatten(1)[:, k // 32:] == 127).all())
+
+
+# ---- a run of them together ------------------------------------------------
+
+class _Decoder:
+    """Two MLP layers and a head on 4-bit weights, as a decode step runs them."""
+
+    def __init__(self, k, hidden, vocab, dtype, seed):
+        self.dtype = dtype
+        self.norms = [(1 + 0.1 * _randn((k,), seed + i)).to(dtype) for i in range(3)]
+
+        def weights(n, k, s):
+            return ops.quantize_mx_fp4(_randn((n, k), s, scale=k ** -0.5))
+
+        self.layers = [(weights(hidden, k, seed + 10 + i), weights(k, hidden, seed + 20 + i))
+                       for i in range(2)]
+        self.head = weights(vocab, k, seed + 30)
+
+    def step(self, x, u, seen=None):
+        note = (lambda *t: None) if seen is None else (lambda *t: seen.append(t))
+        h = None
+        for (up, down), w in zip(self.layers, self.norms):
+            out = ops.rmsnorm_mx(x, w, residual=h)
+            q, sc = out[:2]
+            note("norm_mx", x, w, h, out)
+            h = x if h is None else out[2]
+            a = ops.gemv_mx_w4(q, sc, *up, bf16_out=True)
+            note("mx", (q, sc), up, a)
+            a = torch.relu(a)
+            x = ops.gemv_w4(a, *down, bf16_out=True).to(self.dtype)
+            note("w4", a, down, x)
+        before = h
+        y, h = ops.rmsnorm(x, self.norms[2], residual=before)
+        note("norm", x, self.norms[2], before, (y, h))
+        logits = ops.gemv_w4(y, *self.head)
+        note("w4", y, self.head, logits)
+        token = ops.sample(logits * 4, u, temperature=0.9, top_k=40, top_p=0.95)
+        note("sample", logits * 4, u, token)
+        return token, logits
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 5, 33])
+def test_decode_step(rows):
+    # each operator against 64 bits on what the one before it gave
+    net = _Decoder(512, 1088, 5003, torch.bfloat16, 100)
+    x, u = _randn((rows, 512), 140, torch.bfloat16), _uniform(rows, 141)
+    seen = []
+    token, _ = net.step(x, u, seen)
+    assert token.shape == (rows,) and bool(((0 <= token) & (token < 5003)).all())
+    for kind, *t in seen:
+        if kind == "norm_mx":
+            y64, h64 = _norm64(t[0], t[1], t[2], 1e-6)
+            q, sc = t[3][:2]
+            s = torch.exp2(_mx_rows(sc, q.shape[1]).double() - 127).repeat_interleave(32, 1)
+            err = (_mx_values(q, sc) - y64).abs()
+            assert bool((err <= torch.maximum(2.0 ** -4 * y64.abs(), s * 2.0 ** -10)
+                         + 2 * NORM_REL * y64.abs()).all())
+            if t[2] is not None:
+                assert _near(t[3][2], h64, 2.0 ** -8 + 2.0 ** -24, torch.bfloat16)
+        elif kind == "norm":
+            y64, h64 = _norm64(t[0], t[1], t[2], 1e-6)
+            assert _near(t[3][0], y64, 2.0 ** -8 + NORM_REL, torch.bfloat16)
+            assert _near(t[3][1], h64, 2.0 ** -8 + 2.0 ** -24, torch.bfloat16)
+        elif kind == "mx":
+            assert _product_ok(t[2], _mx_values(*t[0]), _fp4_values(*t[1]))
+        elif kind == "w4":
+            assert _product_ok(t[2], t[0].double(), _fp4_values(*t[1]))
+        else:
+            assert _same_tokens(t[2], t[0], t[1], temperature=0.9, top_k=40, top_p=0.95)
+
+
+@gpu
+def test_decode_step_captured_and_on_two_streams():
+    net = _Decoder(512, 1088, 5003, torch.bfloat16, 200)
+    x, u = _randn((6, 512), 240, torch.bfloat16), _uniform(6, 241)
+    net.step(x, u)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        token, logits = net.step(x, u)
+    for i in range(4):
+        x.copy_(_randn((6, 512), 250 + i, torch.bfloat16))
+        u.copy_(_uniform(6, 260 + i))
+        g.replay()
+        want = net.step(x, u)
+        torch.cuda.synchronize()
+        assert torch.equal(token, want[0]) and torch.equal(logits, want[1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    xs = [_randn((6, 512), 270 + i, torch.bfloat16) for i in range(2)]
+    want = [net.step(v, u) for v in xs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(net.step(xs[i], u))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(t, want[i][0]) and torch.equal(v, want[i][1]) for t, v in got[i])
