@@ -461,15 +461,16 @@ struct RowPick {
     typedef T V __attribute__((ext_vector_type(VEC)));
     // the bins as an interval, so that a logit takes two comparisons
     const float low = bin_begin(r, to);
-    const float above = bin_of(r, r.hi) < from ? bin_begin(r, from - 1) : __builtin_inff();
-    const bool top = above == __builtin_inff();  // which then belongs to it
+    const float high = bin_of(r, r.hi) < from
+                           ? logit_of(order_of(bin_begin(r, from - 1), 0) + (1ull << 32))
+                           : __builtin_inff();  // the next lower logit
     const int lane = (int)threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // Each wave has a list of its own and knows its length: no atomic, whose
     // answer would have to be waited for. All lanes come here together.
     int have = 0;
     auto add = [&](bool there, int i, float x) {
-      const bool in = there && low <= x && (x < above || top);
+      const bool in = there && low <= x && x <= high;
       const u64 who = __ballot(in);
       if (!who) return;
       const int at = have + (int)__builtin_amdgcn_mbcnt_hi(
@@ -492,12 +493,13 @@ struct RowPick {
 #pragma unroll
       for (int l = 0; l < AHEAD; ++l)
         v[l] = body[min(v0 + l * ROW_THREADS + lane, vecs - 1)];
+      const bool all = v0 + (AHEAD - 1) * ROW_THREADS + 64 <= vecs;
 #pragma unroll
       for (int l = 0; l < AHEAD; ++l) {
         const int at = v0 + l * ROW_THREADS + lane;
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          add(at < vecs, head + at * VEC + j, as_f32(v[l][j]));
+          add(all || at < vecs, head + at * VEC + j, as_f32(v[l][j]));
       }
     }
     if (lane == 0) sh.listed[wave] = have;
@@ -651,11 +653,23 @@ __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   const int bin = t % BINS;
   u64 m = 0, minp = 0;
   unsigned n = 0;
-#pragma unroll 4
-  for (int i = t / BINS; i < a.chunks; i += ROW_THREADS / BINS) {
-    m += c[i].mass[bin];
-    n += c[i].count[bin];
-    if (bin == 0) minp += c[i].minp;
+  for (int i0 = t / BINS; i0 < a.chunks; i0 += 4 * (ROW_THREADS / BINS)) {
+    u64 mass[4], least[4];
+    unsigned count[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // all on their way at once
+      const ChunkBins& b = c[min(i0 + j * (ROW_THREADS / BINS), a.chunks - 1)];
+      mass[j] = b.mass[bin];
+      count[j] = b.count[bin];
+      least[j] = b.minp;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j * (ROW_THREADS / BINS) >= a.chunks) break;
+      m += mass[j];
+      n += count[j];
+      minp += least[j];
+    }
   }
   clear(sh.row);
   const RowScale r = row_scale(a, row, row_extent(a, row));
