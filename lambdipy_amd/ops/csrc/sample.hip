@@ -19,9 +19,10 @@
 //
 // f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
 // bin that holds a border, and only that bin's members are looked at. An exp
-// a logit in 64 bits, 33 instructions, is what that takes. Short rows in one
-// workgroup each; long ones as chunks (maxima, then histograms) and one
-// workgroup a row for the borders: 24 x 50001 28 us, 256 x 131072 98 us.
+// a logit in 64 bits, 33 instructions, is what that takes; the instructions
+// bound it. Short rows in one workgroup each; long ones as chunks (maxima,
+// then histograms) and one workgroup a row for the borders: 24 x 50001 27 us,
+// 256 x 131072 96 us.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -37,10 +38,10 @@ constexpr int CHUNK_THREADS = 256;
 constexpr int ROW_THREADS = 1024;
 constexpr int LIST = 512;   // members of bins that a wave keeps in LDS
 constexpr int FEW = 64;     // members that one wave ranks
-// Rows up to here are one workgroup's
-// (16 bits: those whose counts of 512 logits fit the table). f32 by measured
-// time: one row of 16000 takes 16 us so and 19 as chunks, of 32000 24 and 22;
-// 256 rows of 32000 30 and 40, of 64000 49 and 58.
+// Rows up to here are one workgroup's: of 16 bits those whose counts of 512
+// logits fit the table, f32 by measured time: one row of 16000 takes 16 us so
+// and 19 as chunks, of 32000 24 and 22; 256 rows of 32000 29 and 40, of 64000
+// 48 and 58.
 constexpr int WHOLE = 24576, WHOLE_MANY = 65536, MANY = 96, WHOLE_16 = 262144;
 
 struct ChunkMax {
@@ -1117,10 +1118,10 @@ struct Plan {
 Plan plan_of(int rows, int vocab, bool half) {
   // At least 4096 logits a chunk; more where there are chunks enough for the
   // chip without that, so that fewer histograms are written.
-  const long want = ((long)rows * vocab + 2047) / 2048;
   Plan p{};
   if (vocab <= (half ? WHOLE_16 : rows >= MANY ? WHOLE_MANY : WHOLE)) return p;
-  p.chunk = (int)(want < 4096 ? 4096 : (want + 511) / 512 * 512);
+  const long want = ((long)rows * vocab + 2047) / 2048;
+  p.chunk = want <= 4096 ? 4096 : (int)(((want < vocab ? want : vocab) + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
   p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
   p.bytes = p.maxima_bytes + (size_t)rows * p.chunks * sizeof(ChunkBins);
