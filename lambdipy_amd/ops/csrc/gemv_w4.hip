@@ -19,8 +19,8 @@
 //
 // Measured: 100000 x 8192 by one bf16 row 73 us, 5.9 TB/s (reading alone
 // reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.4 us; 28000 x 8192 by 64
-// MX rows 44 us, where the MFMA (27% busy) and the conversions to bf16 take
-// more than the memory.
+// MX rows 44 us, where the MFMA (27% busy), the conversions to bf16, LDS and the
+// load path take about a quarter of the time each, one after another.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -117,11 +117,13 @@ struct Step {
 template <int MODE, int MT, int NT, bool FEW>
 struct Exchange {
   static constexpr int XTILE = Step<MODE, MT, NT, FEW>::XL * 1024;
-  static constexpr int XTILES = MT < 2 ? MT : 2;  // taken in turn
   static_assert(NT <= 4 && MT <= 4, "a lane brings one scale of each side");
+  // In LDS the scales cost less than between lanes, but 64 rows of 16 bits
+  // leave no room for them where two workgroups are to share a CU's 160 KB.
+  static constexpr bool SCALES = MODE == X_MX || MT < 4;
   unsigned char w[NT][1024];
-  unsigned char x[XTILES][XTILE];
-  unsigned sw[NT * 16], sx[MT * 16];
+  unsigned char x[MT][XTILE];
+  unsigned sw[SCALES ? NT * 16 : 0], sx[MODE == X_MX ? MT * 16 : 0];
 };
 
 // MT x NT tiles of 16 rows of x by 16 rows of weights.
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
   // branch, so that the compiler's waits count them: turns behind the last
   // step read that one again, and where K ends in the middle of the last
   // step, the second half of the pieces reads the first half again.
-  // `multiply` clears what was read in place of nothing.
+  // `turn_round` clears what was read in place of nothing.
   const int turns = (steps + WAVES - 1) / WAVES;
   auto load = [&](S& f, int turn) {
     const int s = min(wave + turn * WAVES, steps - 1);
@@ -209,64 +211,89 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
                         : (row * 16 + (piece ^ row)) * 16;
   };
 
-  auto multiply = [&](const S& f, int turn) {
+  // What a lane multiplies: its block of each tile's rows, as loaded.
+  struct Turned {
+    i32x4 w[NT], x[MT][MODE == X_MX ? 2 : 4];
+    unsigned sw[NT], sx[MT];
+  };
+  auto turn_round = [&](const S& f, Turned& q, int turn) {
     const int s = wave + turn * WAVES;
     const bool none = s >= steps;
     const bool part = none || (half_last && s == steps - 1);
     const i32x4 zero = {0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < NT; ++t) put(ex.w[t] + wat(lane / WROW, lane % WROW), f.w[t]);
-    ex.sw[lane % (NT * 16)] = part ? f.sw & 0xffffu : f.sw;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int l = 0; l < S::XL; ++l)
+        put(ex.x[i] + xat(l * (64 / XROW) + lane / XROW, lane % XROW), f.x[i][l]);
+    const unsigned sw = part ? f.sw & 0xffffu : f.sw;
+    if constexpr (E::SCALES) ex.sw[lane % (NT * 16)] = sw;
     if constexpr (MODE == X_MX)
       ex.sx[lane % (MT * 16)] = part ? f.sx & 0xffffu : f.sx;
     in_order();
-    i32x4 w[NT];
-    unsigned sw[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      w[t] = get(ex.w[t] + wat(c, g));
-      sw[t] = ex.sw[t * 16 + c];
-      if (part && (none || g >= 2)) w[t] = zero;
+      q.w[t] = get(ex.w[t] + wat(c, g));
+      if constexpr (E::SCALES)
+        q.sw[t] = ex.sw[t * 16 + c];
+      else
+        q.sw[t] = (unsigned)__shfl((int)sw, t * 16 + c, 64);
     }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (MODE == X_MX) {
+        // a lane's block lies in the pieces of two quarters
+        const int at = (g >> 1) * 4 + (g & 1);
+        q.x[i][0] = get(ex.x[i] + xat(xc, at));
+        q.x[i][1] = get(ex.x[i] + xat(xc, at + 2));
+        q.sx[i] = ex.sx[i * 16 + c];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q.x[i][j] = get(ex.x[i] + xat(xc, MODE == X_F16 ? 4 * j + g : 4 * g + j));
+      }
+    }
+    in_order();
+    if (part) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (none || g >= 2) q.w[t] = zero;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < (MODE == X_MX ? 2 : 4); ++j)
+          if (none || (MODE == X_F16 ? j >= 2 : g >= 2)) q.x[i][j] = zero;
+    }
+  };
+
+  auto multiply = [&](Turned& q) {
     // 16-bit weights, once for all rows of x
     i32x4 b[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      if constexpr (MODE == X_F16) w[t] = transpose_groups(w[t]);
+      if constexpr (MODE == X_F16) q.w[t] = transpose_groups(q.w[t]);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         b[t][j] = MODE == X_F16
-                      ? __builtin_bit_cast(i32x4, w_f16(w[t][j]))
-                      : __builtin_bit_cast(i32x4, w_bf16(w[t][j], scale_of(sw[t], g)));
+                      ? __builtin_bit_cast(i32x4, w_f16(q.w[t][j]))
+                      : __builtin_bit_cast(i32x4, w_bf16(q.w[t][j], scale_of(q.sw[t], g)));
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      unsigned char* const xs = ex.x[i % E::XTILES];
-#pragma unroll
-      for (int l = 0; l < S::XL; ++l)
-        put(xs + xat(l * (64 / XROW) + lane / XROW, lane % XROW), f.x[i][l]);
-      in_order();
       i32x4 x[4];
       if constexpr (MODE == X_MX) {
-        // a lane's block lies in the pieces of two quarters
-        const int q = (g >> 1) * 4 + (g & 1);
-        const i32x4 lo = get(xs + xat(xc, q)), hi = get(xs + xat(xc, q + 2));
-        const float sx = scale_of(ex.sx[i * 16 + c], g);
+        const i32x4 lo = q.x[i][0], hi = q.x[i][1];
+        const float sx = scale_of(q.sx[i], g);
         x[0] = __builtin_bit_cast(i32x4, x_bf16(lo[0], lo[1], sx));
         x[1] = __builtin_bit_cast(i32x4, x_bf16(lo[2], lo[3], sx));
         x[2] = __builtin_bit_cast(i32x4, x_bf16(hi[0], hi[1], sx));
         x[3] = __builtin_bit_cast(i32x4, x_bf16(hi[2], hi[3], sx));
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[j] = get(xs + xat(xc, MODE == X_F16 ? 4 * j + g : 4 * g + j));
+        for (int j = 0; j < 4; ++j) x[j] = q.x[i][j];
       }
-      if (part) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (none || (MODE == X_F16 ? j >= 2 : g >= 2)) x[j] = zero;
-      }
-      in_order();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -278,7 +305,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
             const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 __builtin_bit_cast(nf16x8, x[j]), __builtin_bit_cast(nf16x8, b[t][j]),
                 f32x4{0, 0, 0, 0}, 0, 0, 0);
-            const float sc = scale_of(sw[t], j);
+            const float sc = scale_of(q.sw[t], j);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               acc[i][t][r] = __builtin_fmaf(p[r], sc, acc[i][t][r]);
@@ -300,13 +327,19 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
   for (; turn + DEPTH < turns; turn += DEPTH) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      multiply(f[d], turn + d);
-      load(f[d], turn + d + DEPTH);
+      Turned q;
+      turn_round(f[d], q, turn + d);
+      load(f[d], turn + d + DEPTH);  // on its way while this one is multiplied
+      multiply(q);
     }
   }
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d)
-    if (turn + d < turns) multiply(f[d], turn + d);
+    if (turn + d < turns) {
+      Turned q;
+      turn_round(f[d], q, turn + d);
+      multiply(q);
+    }
 
   // Join the waves' sums; then a thread owns four rows of one column.
   __syncthreads();
@@ -349,8 +382,8 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
 // but with fewer than one workgroup a CU the rest of the chip is idle. Over
 // M = 12 .. 64 and N x K from 1000 x 2048 to 100000 x 8192 this is the
 // fastest of the sixteen shapes tried or within a tenth of it (8192 x 8192,
-// M = 64 MX: 32 x 64 tiles on 256 workgroups 15.0 us, 64 x 64 on 128 more
-// than 19.6; 28000 x 8192: 56 and 44 us).
+// M = 64 MX: 32 x 64 tiles on 256 workgroups 12.7 us, 64 x 64 on 128 18.0;
+// 28000 x 8192: 55 and 44 us).
 template <int MODE>
 hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
