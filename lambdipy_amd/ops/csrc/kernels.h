@@ -273,6 +273,8 @@ struct SampleParam {
 // token[r]: drawn from row r of logits [rows, vocab] (row stride in elements)
 // by u[r] after temperature, top-k, top-p and min-p; -1 where a row has no
 // logit over -inf. workspace: sample_workspace(t, rows, vocab) bytes.
+// 16-bit rows: at most SAMPLE_MOST_16 logits (longer ones as f32).
+constexpr int SAMPLE_MOST_16 = 524288;
 size_t sample_workspace(ActType t, int rows, int vocab);
 hipError_t sample(ActType t, const void* logits, long stride, int rows,
                   int vocab, SampleParam temperature, SampleParam top_k,

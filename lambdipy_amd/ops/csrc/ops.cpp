@@ -963,10 +963,11 @@ lpx::SampleParam setting(const Setting& v, const char* name, int64_t rows, bool 
                                : lpx::SampleParam::f64};
 }
 
-at::Tensor sample(const at::Tensor& logits, const at::Tensor& u, const Setting& temperature,
+at::Tensor sample(const at::Tensor& all, const at::Tensor& u, const Setting& temperature,
                   const Setting& top_k, const Setting& top_p, const Setting& min_p) {
+  at::Tensor logits = all;
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1, "sample expects logits [..., V], V >= 1");
-  const auto type = act_type(logits, "sample");
+  auto type = act_type(logits, "sample");
   const int64_t V = logits.size(-1), rows = logits.numel() / V;
   TORCH_CHECK(V <= (1 << 24) && rows < (int64_t(1) << 31), "sample: too large");
   std::vector<at::Tensor> keep;
@@ -978,6 +979,10 @@ at::Tensor sample(const at::Tensor& logits, const at::Tensor& u, const Setting& 
   const auto draw = setting(u, "u", rows, false, 0, 1, logits, keep);
   TORCH_CHECK(logits.is_cuda(), "sample: logits must be on the ROCm device (got CPU)");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  if (type != lpx::ActType::f32 && V > lpx::SAMPLE_MOST_16) {
+    logits = logits.to(at::kFloat);
+    type = lpx::ActType::f32;
+  }
   const at::Tensor x = dense_rows(logits);
   auto token = fresh(logits.sizes().slice(0, logits.dim() - 1), at::kLong, logits);
   const auto bytes = (int64_t)lpx::sample_workspace(type, (int)rows, (int)V);

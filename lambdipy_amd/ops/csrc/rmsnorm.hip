@@ -7,7 +7,7 @@
 //       max|y| / 2^e <= 448; payload e4m3(y / 2^e), scale byte e + 127
 //
 // The norm is taken of the unrounded f32 sum, y is rounded once, and the sum
-// of squares is held in f32 (at most 64 terms a thread, then a tree).
+// of squares is held in f32 (a thread's terms in turn, then a tree).
 //
 // The row stays in registers between the two uses of it, so each input is
 // read once and each output written once; memory bounds it. A thread owns 8
@@ -246,8 +246,6 @@ hipError_t launch(const NormArgs& a, hipStream_t stream) {
     rmsnorm_kernel<T, MX, 1><<<grid, block, 0, stream>>>(a);
   else if (threads <= 2048)
     rmsnorm_kernel<T, MX, 2><<<grid, most, 0, stream>>>(a);
-  else if (threads <= 4096)
-    rmsnorm_kernel<T, MX, 4><<<grid, most, 0, stream>>>(a);
   else
     rmsnorm_long_kernel<T, MX><<<grid, most, 0, stream>>>(a);
   return hipGetLastError();

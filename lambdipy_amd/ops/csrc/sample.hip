@@ -14,8 +14,9 @@
 //
 // 16-bit rows: one workgroup a row counts each of the 65536 values in LDS and
 // looks the borders up among them; the exps are as many as the values that
-// occur. 256 x 131072 bf16: 34 us (the LDS atomics of the counting take 10,
-// reading the row a second time for the index 8); 1 x 32000: 15 us.
+// occur. 256 x 131072 bf16: 36 us (the LDS atomics of the counting take 10,
+// reading the row a second time for the index 8), 38 where 9 of 10 are masked;
+// 1 x 32000: 15 us; 1 x 524288: 67 (115 as f32).
 //
 // f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
 // bin that holds a border, and only that bin's members are looked at. An exp
@@ -38,11 +39,10 @@ constexpr int CHUNK_THREADS = 256;
 constexpr int ROW_THREADS = 1024;
 constexpr int LIST = 512;   // members of bins that a wave keeps in LDS
 constexpr int FEW = 64;     // members that one wave ranks
-// Rows up to here are one workgroup's: of 16 bits those whose counts of 512
-// logits fit the table, f32 by measured time: one row of 16000 takes 16 us so
-// and 19 as chunks, of 32000 24 and 22; 256 rows of 32000 29 and 40, of 64000
-// 48 and 58.
-constexpr int WHOLE = 24576, WHOLE_MANY = 65536, MANY = 96, WHOLE_16 = 262144;
+// f32 rows up to here are one workgroup's, by measured time: one row of 16000
+// takes 16 us so and 19 as chunks, of 32000 24 and 22; 256 rows of 32000 29
+// and 40, of 64000 48 and 58.
+constexpr int WHOLE = 24576, WHOLE_MANY = 65536, MANY = 96;
 
 struct ChunkMax {
   float hi, lo;  // largest; smallest that is not -inf
@@ -282,8 +282,10 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_max_kernel(SampleArgs a) 
 
 // ---- 2: histograms --------------------------------------------------------
 
-// Adds [begin, end) of a row to bins in LDS. Counts are only asked for where
-// the row is cut by top-k or top-p.
+// Adds [begin, end) of a row to bins in LDS: the logits that have a weight.
+// (The others follow them all, and cutting among those changes nothing. Where
+// a mask is the type's lowest value they are most of a row, in one bin.)
+// Counts are only asked for where the row is cut by top-k or top-p.
 template <int THREADS, typename T, typename B>
 __device__ __forceinline__ void add_bins(B& b, const RowScale& r, u64 least,
                                          const T* row, int begin, int end) {
@@ -292,8 +294,10 @@ __device__ __forceinline__ void add_bins(B& b, const RowScale& r, u64 least,
   scan<THREADS, 2>(row, begin, end, [&](int, float x) {
     const int bin = bin_of(r, x);
     const u64 w = weight(r, x);
-    if (counted && real(x)) atomicAdd(&b.count[bin], 1u);
-    if (w) atomicAdd(&b.mass[bin], w);
+    if (w) {
+      if (counted) atomicAdd(&b.count[bin], 1u);
+      atomicAdd(&b.mass[bin], w);
+    }
     minp += w >= least ? w : 0;
   });
 #pragma unroll
@@ -456,8 +460,7 @@ struct RowPick {
   }
 
   // Lists the members of bins [from, to], unless a wave's are too many.
-  // Returns how many they are.
-  __device__ __forceinline__ unsigned collect(int from, int to) {
+  __device__ __forceinline__ void collect(int from, int to) {
     constexpr int VEC = 16 / sizeof(T), AHEAD = 4;
     typedef T V __attribute__((ext_vector_type(VEC)));
     // the bins as an interval, so that a logit takes two comparisons
@@ -515,23 +518,26 @@ struct RowPick {
     first = from;
     last = fits ? to : from - 1;
     found = all;
-    return all;
   }
 
   // The member of the row at which the running count (mass) reaches `border`:
-  // its index to sh.at, the running mass with it to sh.mass.
-  __device__ __forceinline__ void resolve(bool by_count, u64 border) {
+  // its index to sh.at, the running mass with it to sh.mass. `more`: borders
+  // further up will be asked for, so that all from the top is listed if it
+  // fits.
+  __device__ __forceinline__ void resolve(bool by_count, u64 border, bool more) {
     const int bin = bin_at(sh.row, by_count, border, sh);
     // what stands before [lo, hi], and how many members that has at most
     unsigned base = bin ? sh.row.count[bin - 1] : 0;
     u64 mass = bin ? sh.row.mass[bin - 1] : 0;
-    unsigned n;
-    if (listed(bin)) {
-      const unsigned members = sh.row.count[bin] - base;
-      n = first == last ? found : members;
-    } else {
-      n = collect(bin, bin);
+    for (int from = more && sh.row.count[bin] <= LIST * 8 ? 0 : bin; !listed(bin);) {
+      collect(from, bin);
+      if (from == bin) break;
+      from = bin;  // that alone, if all does not fit
+      __syncthreads();
     }
+    // (bins are counted where more than one is listed)
+    unsigned n = first == bin && (last == bin || !listed(bin)) ? found
+                                                               : sh.row.count[bin] - base;
     u64 lo = 0, hi = ~0ull;
     while (n > FEW) {
       // 256 sub-bins between the first and the last member; the two differ,
@@ -562,9 +568,10 @@ struct RowPick {
       const int drop = max(0, 64 - __clzll((long long)(hi - lo)) - 8);
       members(bin, lo, hi, [&](u64 o, float x) {
         const int s = (int)((o - lo) >> drop);
-        atomicAdd(&sh.sub.count[s], 1u);
         const u64 w = weight(r, x);
-        if (w) atomicAdd(&sh.sub.mass[s], w);
+        if (!w) return;
+        atomicAdd(&sh.sub.count[s], 1u);
+        atomicAdd(&sh.sub.mass[s], w);
       });
       __syncthreads();
       run_up(sh.sub, sh);
@@ -584,8 +591,10 @@ struct RowPick {
     }
     __syncthreads();
     members(bin, lo, hi, [&](u64 o, float x) {
+      const u64 w = weight(r, x);
+      if (!w) return;
       const int i = atomicAdd(&sh.found, 1);
-      if (i < FEW) sh.few[i] = Member{o, weight(r, x)};
+      if (i < FEW) sh.few[i] = Member{o, w};
     });
     __syncthreads();
     if (threadIdx.x < 64) {
@@ -622,26 +631,21 @@ __device__ __forceinline__ int pick_token(const SampleArgs& a, int row,
 
   u64 kept = total;
   const double k = param(a.top_k, row);
-  if (r.by_k && k < (double)all) {
-    const unsigned want = (unsigned)k;
-    const int bin = bin_at(sh.row, true, want, sh);
-    if (sh.row.count[bin] <= LIST * 8) pick.collect(0, bin);
-    if (sh.row.count[bin] == want) {
-      kept = sh.row.mass[bin];
+#pragma unroll 1  // one copy of the code for the three borders
+  for (int cut = 0; cut < 3; ++cut) {
+    u64 border;
+    if (cut == 0) {
+      if (!(r.by_k && k < (double)all)) continue;
+      border = (u64)k;
+    } else if (cut == 1) {
+      if (!r.by_p) continue;
+      border = share_of(param(a.top_p, row), kept);
     } else {
-      pick.resolve(true, want);
-      kept = sh.mass;
+      border = draw_border(param(a.u, row), min(kept, sh.row.minp));
     }
-  }
-  if (r.by_p) {
-    const u64 border = share_of(param(a.top_p, row), kept);
-    const int bin = bin_at(sh.row, false, border, sh);
-    if (!pick.listed(bin) && sh.row.count[bin] <= LIST * 8) pick.collect(0, bin);
-    pick.resolve(false, border);
+    pick.resolve(cut == 0, border, cut < 2);
     kept = sh.mass;
   }
-  kept = min(kept, sh.row.minp);
-  pick.resolve(false, draw_border(param(a.u, row), kept));
   return sh.at;
 }
 
@@ -735,6 +739,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
 // that of -inf on are -inf and NaN.
 
 constexpr int GROUPS = 1024;  // of 64 neighbouring ranks
+static_assert(SAMPLE_MOST_16 == GROUPS * 512, "a row's counts of 512 logits");
 
 template <typename T> struct Ranks;
 template <> struct Ranks<__bf16> {
@@ -759,7 +764,9 @@ __device__ __forceinline__ unsigned ranks_of(unsigned two) {
 struct TableShared {
   // Rank r's count is in half r >> 15 of word r & 0x7fff. A count of 65536
   // and more runs over; the counts' sum then falls short of the row's length.
+  // A lowest value that is often there, a mask's say, has a count of its own.
   unsigned count[32768];
+  unsigned last, lowest;   // that value's rank (0: none) and count
   u64 mass[GROUPS];        // of 64 ranks; running sums later
   unsigned members[GROUPS];  // counted for top-k; later for 512 logits each
   u64 wave_sum[ROW_THREADS / 64], wave_sum2[ROW_THREADS / 64];
@@ -772,36 +779,28 @@ struct TableShared {
   int token;
 };
 
-// f(index of the first, 8 values) / g(index, value) for a row's 16-bit words.
-template <int AHEAD, typename F, typename G>
-__device__ __forceinline__ void scan_words(const unsigned short* row, int n,
-                                           F f, G g) {
-  const int t = (int)threadIdx.x;
-  const int off = (int)(((uintptr_t)row & 15) / 2);
-  const int head = min(off ? 8 - off : 0, n);
-  if (t < head) g(t, (unsigned)row[t]);
-  const int vecs = (n - head) / 8;
-  const i32x4* body = reinterpret_cast<const i32x4*>(row + head);
-  for (int i = t; i < vecs; i += AHEAD * ROW_THREADS) {
-    i32x4 v[AHEAD];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (i + a * ROW_THREADS < vecs) v[a] = body[i + a * ROW_THREADS];
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
-      if (i + a * ROW_THREADS < vecs) f(head + (i + a * ROW_THREADS) * 8, v[a]);
-  }
-  const int tail = head + vecs * 8 + t;
-  if (tail < n) g(tail, (unsigned)row[tail]);
-}
-
 template <typename T>
 __device__ __forceinline__ float logit_at(unsigned rank) {
   return Ranks<T>::value((rank >> 15 ? rank : 0x7fffu - rank) & 0xffffu);
 }
 
 __device__ __forceinline__ unsigned count_at(const TableShared& sh, unsigned rank) {
+  if (rank == sh.last) return sh.lowest;
   return (sh.count[rank & 0x7fff] >> (rank >> 15 ? 16 : 0)) & 0xffffu;
+}
+
+// The largest of the wave's lanes.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#define LPX_MAX_FROM(ctrl, rows)                                                   \
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false));
+  LPX_MAX_FROM(0x111, 0xf)  // row_shr 1, 2, 4, 8; row_bcast 15 and 31
+  LPX_MAX_FROM(0x112, 0xf)
+  LPX_MAX_FROM(0x114, 0xf)
+  LPX_MAX_FROM(0x118, 0xf)
+  LPX_MAX_FROM(0x142, 0xa)
+  LPX_MAX_FROM(0x143, 0xc)
+#undef LPX_MAX_FROM
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // The value at which the running count (mass) reaches `border`, which of its
@@ -939,7 +938,8 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
     __device__ Shared() {}
   } shared;
   TableShared& sh = shared.table;
-  const int row = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int row = (int)blockIdx.x, t = (int)threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const unsigned short* x = static_cast<const unsigned short*>(a.logits) + row * a.stride;
   const bool greedy = !(param(a.temperature, row) > 0);
 
@@ -952,6 +952,8 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
     sh.members[t] = 0;
     if (t == 0) {
       sh.first = 0xffffu;
+      sh.last = 0;
+      sh.lowest = 0;
       sh.logits = 0;
       sh.minp = 0;
       sh.group = 0;
@@ -971,29 +973,81 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
                         u16x2{(unsigned short)Ranks<T>::INF, (unsigned short)Ranks<T>::INF};
     lows = __builtin_elementwise_min(lows, above);
   };
-  auto one = [&](unsigned rank) {
-    if (!greedy) atomicAdd(&sh.count[rank & 0x7fff], 1u << (rank >> 15 << 4));
+  auto add = [&](unsigned rank, unsigned n) {
+    atomicAdd(&sh.count[rank & 0x7fff], n << (rank >> 15 << 4));
   };
-  scan_words<4>(
-      x, a.vocab,
-      [&](int, i32x4 v) {
+  // Atomics on one word wait for each other: a masked row of 32000 took 37 us
+  // by them. So where the lowest of the 2048 logits that a wave holds is in
+  // many of its lanes, they count it in a register.
+  unsigned last = 0, lowest = 0;
+  constexpr int AHEAD = 4, MANY_LANES = 8;
+  const int vocab = a.vocab;
+  const int off = (int)(((uintptr_t)x & 15) / 2);
+  const int head = min(off ? 8 - off : 0, vocab);
+  const int vecs = (vocab - head) / 8;
+  const i32x4* body = reinterpret_cast<const i32x4*>(x + head);
+  if (t < 16) {  // the ends
+    const int at = t < 8 ? t : head + vecs * 8 + t - 8;
+    if (at < (t < 8 ? head : vocab)) {
+      const unsigned two = ranks_of((unsigned)x[at] * 0x10001u);
+      highest(two);
+      if (!greedy) add(two & 0xffffu, 1u);
+    }
+  }
+  for (int v0 = wave * 64; v0 < vecs; v0 += AHEAD * ROW_THREADS) {
+    i32x4 v[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const unsigned two = ranks_of((unsigned)v[j]);
-          highest(two);
-          one(two & 0xffffu);
-          one(two >> 16);
+    for (int l = 0; l < AHEAD; ++l)
+      if (v0 + l * ROW_THREADS < vecs)
+        v[l] = body[min(v0 + l * ROW_THREADS + lane, vecs - 1)];
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int l = 0; l < AHEAD; ++l) {
+      if (v0 + l * ROW_THREADS >= vecs) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[l][j] = (int)ranks_of((unsigned)v[l][j]);
+        highest((unsigned)v[l][j]);
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[l][j]));
+      }
+    }
+    if (greedy) continue;
+    const unsigned own = min(max((unsigned)most[0], (unsigned)most[1]), Ranks<T>::NONE);
+    const unsigned far = wave_max(own);
+    const bool often = far >= last && __popcll(__ballot(own == far)) >= MANY_LANES;
+    if (often && far > last) {
+      if (lowest) add(last, lowest);
+      last = far;
+      lowest = 0;
+    }
+#pragma unroll
+    for (int l = 0; l < AHEAD; ++l) {
+      const int at = v0 + l * ROW_THREADS;
+      if (at >= vecs) break;
+      if (at + lane >= vecs) continue;
+      if (often) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const unsigned rank = (unsigned)v[l][j / 2] >> (j % 2 * 16) & 0xffffu;
+          if (rank == last)
+            ++lowest;
+          else
+            add(rank, 1u);
         }
-      },
-      [&](int, unsigned bits) {
-        const unsigned two = ranks_of(bits << 16 | bits);
-        highest(two);
-        one(two & 0xffffu);
-      });
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          add((unsigned)v[l][j / 2] >> (j % 2 * 16) & 0xffffu, 1u);
+      }
+    }
+  }
   unsigned low = min((unsigned)lows[0], (unsigned)lows[1]);
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) low = min(low, (unsigned)__shfl_xor(low, m, 64));
-  if (lane == 0) atomicMin(&sh.first, low);
+  if (lane == 0) {
+    atomicMin(&sh.first, low);
+    atomicMax(&sh.last, last);
+  }
   __syncthreads();
   unsigned first = sh.first + Ranks<T>::INF;
   if (first >= Ranks<T>::NONE) {  // nothing over -inf
@@ -1006,14 +1060,32 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
     if (t == 0) a.token[row] = token;
     return;
   }
-  if (t == 0) {  // -0 is 0
-    const unsigned both = sh.count[0x7fff] & 0xffffu, minus = sh.count[0] >> 16;
-    if (both + minus < 65536u) {
-      sh.count[0x7fff] += minus;
-      sh.count[0] &= 0xffffu;
-    } else {
-      sh.count[0x7fff] &= 0xffff0000u;  // too many: the sum will say so
+  {
+    const unsigned n = (unsigned)wave_run_up((u64)lowest);
+    if (lane == 63 && n) {
+      if (last == sh.last)
+        atomicAdd(&sh.lowest, n);
+      else
+        add(last, n);
     }
+  }
+  __syncthreads();
+  if (t == 0) {
+    // -0 is 0
+    const unsigned plus = sh.count[0x7fff] & 0xffffu, minus = sh.count[0] >> 16;
+    sh.count[0] &= 0xffffu;
+    if (sh.last == 0x8000u) sh.last = 0x7fffu;
+    if (sh.last == 0x7fffu)
+      sh.lowest += minus;
+    else if (plus + minus < 65536u)
+      sh.count[0x7fff] += minus;
+    else
+      sh.count[0x7fff] &= 0xffff0000u;  // too many: the sum will say so
+    // all of the lowest together; its place in the table says that there is one
+    const unsigned at = sh.last & 0x7fff, half = sh.last >> 15 << 4;
+    sh.lowest += sh.count[at] >> half & 0xffffu;
+    sh.count[at] = (sh.count[at] & ~(0xffffu << half)) | 1u << half;
+    sh.logits = sh.lowest - 1u;
   }
   __syncthreads();
 
@@ -1039,6 +1111,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
       const int group = b * 4 + (j & 3) + (j >> 2) * (GROUPS / 2);
       const unsigned rank = (unsigned)group * 64 + lane;
       unsigned n = j >> 2 ? two[j & 3] >> 16 : two[j & 3] & 0xffffu;
+      if (rank == sh.last) n = sh.lowest;
       if (rank < Ranks<T>::INF || rank >= Ranks<T>::NONE) n = 0;
       if (!__ballot(n != 0)) continue;
       const u64 w = weight(r, logit_at<T>(rank));
@@ -1096,17 +1169,16 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
 template <typename T>
 hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   const dim3 rows((unsigned)a.rows), threads(ROW_THREADS);
-  if (a.chunks == 0) {
-    if constexpr (sizeof(T) == 2)
-      row_table_kernel<T><<<rows, threads, 0, stream>>>(a);
-    else
-      row_whole_kernel<T><<<rows, threads, 0, stream>>>(a);
-    return hipGetLastError();
+  if constexpr (sizeof(T) == 2) {
+    row_table_kernel<T><<<rows, threads, 0, stream>>>(a);
+  } else if (a.chunks == 0) {
+    row_whole_kernel<T><<<rows, threads, 0, stream>>>(a);
+  } else {
+    const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
+    chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+    chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+    row_pick_kernel<T><<<rows, threads, 0, stream>>>(a);
   }
-  const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
-  chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
-  chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
-  row_pick_kernel<T><<<rows, threads, 0, stream>>>(a);
   return hipGetLastError();
 }
 
@@ -1115,11 +1187,11 @@ struct Plan {
   size_t maxima_bytes, bytes;
 };
 
-Plan plan_of(int rows, int vocab, bool half) {
+Plan plan_of(ActType t, int rows, int vocab) {
   // At least 4096 logits a chunk; more where there are chunks enough for the
   // chip without that, so that fewer histograms are written.
   Plan p{};
-  if (vocab <= (half ? WHOLE_16 : rows >= MANY ? WHOLE_MANY : WHOLE)) return p;
+  if (t != ActType::f32 || vocab <= (rows >= MANY ? WHOLE_MANY : WHOLE)) return p;
   const long want = ((long)rows * vocab + 2047) / 2048;
   p.chunk = want <= 4096 ? 4096 : (int)(((want < vocab ? want : vocab) + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
@@ -1131,7 +1203,7 @@ Plan plan_of(int rows, int vocab, bool half) {
 }  // namespace
 
 size_t sample_workspace(ActType t, int rows, int vocab) {
-  return rows > 0 && vocab > 0 ? plan_of(rows, vocab, t != ActType::f32).bytes : 0;
+  return rows > 0 && vocab > 0 ? plan_of(t, rows, vocab).bytes : 0;
 }
 
 hipError_t sample(ActType t, const void* logits, long stride, int rows,
@@ -1140,7 +1212,8 @@ hipError_t sample(ActType t, const void* logits, long stride, int rows,
                   void* workspace, int64_t* token, hipStream_t stream) {
   if (rows <= 0) return hipSuccess;
   if (vocab <= 0) return hipErrorInvalidValue;
-  const Plan p = plan_of(rows, vocab, t != ActType::f32);
+  if (t != ActType::f32 && vocab > SAMPLE_MOST_16) return hipErrorInvalidValue;
+  const Plan p = plan_of(t, rows, vocab);
   if ((int64_t)rows * p.chunks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
   int shift = 45;  // sums of `vocab` weights stay below 2^62
   while (vocab > (int64_t(1) << (62 - shift))) --shift;

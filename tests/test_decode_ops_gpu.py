@@ -868,3 +868,46 @@ def test_decode_step_captured_and_on_two_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(t, want[i][0]) and torch.equal(v, want[i][1]) for t, v in got[i])
+
+
+# As SAMPLE_NEAR for 2^19 + 1 logits, whose weights are held in steps of 2^-42
+LONG_NEAR = 2 * (2.0 ** 19.1 * 2.0 ** -43 + 2.0 ** -44)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("v", [524288, 524289])
+def test_sample_the_longest_16_bit_rows(dtype, v):
+    # up to 2^19 by the counts of values, above as f32
+    x = _randn((2, v), 83, dtype, 2.0)
+    x[0, v - 1] = 40.0
+    for st in (dict(top_k=20), dict(temperature=0.0), dict(top_p=0.5)):
+        u = _uniform(2, 84)
+        got = ops.sample(x, u, **st).cpu()
+        want, near = _sample64(x, u, **st)
+        far = near > LONG_NEAR
+        assert torch.equal(got[far], want[far]) and int(got[0]) == v - 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", [-torch.inf, "lowest", -1e4, 0.0, -0.0, torch.nan])
+@pytest.mark.parametrize("settings", [
+    {}, dict(top_k=50), dict(top_k=120000), dict(top_p=0.9), dict(min_p=0.05),
+    dict(top_k=40, top_p=0.5, temperature=0.7), dict(temperature=0.0)])
+def test_sample_rows_that_are_mostly_masked(dtype, mask, settings):
+    v = 131075
+    x = _randn((6, v), 85, dtype, 2.0)
+    if mask == 0.0:
+        x = x.abs()  # the masked are the lowest
+    m = torch.finfo(dtype).min if mask == "lowest" else mask
+    gen = torch.Generator(device="cuda").manual_seed(86)
+    there = torch.rand((6, v), generator=gen, device="cuda")
+    x[0] = torch.where(there[0] < 0.9, m, x[0])
+    x[1] = torch.where(there[1] < 0.5, m, x[1])
+    x[2] = torch.where(there[2] < 0.9999, m, x[2])
+    x[3] = m  # every one
+    x[4, 17:] = m
+    x[5] = torch.where(there[5] < 0.6, m, -m if mask == 0.0 else x[5])
+    u = _uniform(6, 87)
+    _same_tokens(ops.sample(x, u, **settings), x, u, **settings)
