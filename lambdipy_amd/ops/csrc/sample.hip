@@ -14,9 +14,10 @@
 //
 // 16-bit rows: one workgroup a row counts each of the 65536 values in LDS and
 // looks the borders up among them; the exps are as many as the values that
-// occur. 256 x 131072 bf16: 36 us (the LDS atomics of the counting take 10,
-// reading the row a second time for the index 8), 38 where 9 of 10 are masked;
-// 1 x 32000: 15 us; 1 x 524288: 67 (115 as f32).
+// occur. 256 x 131072 bf16: 33 us, 32 where 9 of 10 are masked, 14 greedy; of
+// the 26 in the kernel the LDS atomics of the counting take 11, reading the
+// row a second time for the index 5, the sums and exps of its 72 groups of 64
+// values 4. 1 x 32000: 15 us; 1 x 524288: 64 (115 as f32).
 //
 // f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
 // bin that holds a border, and only that bin's members are looked at. An exp
@@ -79,15 +80,20 @@ __device__ __forceinline__ float as_f32(float x) { return x; }
 __device__ __forceinline__ float as_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float as_f32(__bf16 x) { return (float)x; }
 
+// Bytes of a load. 16-bit rows come here seldom, and their kernel has no
+// registers for more.
+template <typename T>
+constexpr int LOAD = sizeof(T) == 2 ? 4 : 16;
+
 // f(index, logit) for every logit of [begin, end). A thread's indices rise.
-// AHEAD: 16-B loads in flight a thread.
+// AHEAD: loads in flight a thread.
 template <int THREADS, int AHEAD, typename T, typename F>
 __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
                                      int end, F f) {
-  constexpr int VEC = 16 / sizeof(T);
+  constexpr int VEC = LOAD<T> / sizeof(T);
   typedef T V __attribute__((ext_vector_type(VEC)));
   const int tid = (int)threadIdx.x;
-  const int off = (int)(((uintptr_t)(row + begin) & 15) / sizeof(T));
+  const int off = (int)((uintptr_t)(row + begin) % LOAD<T> / sizeof(T));
   const int head = min(off ? VEC - off : 0, end - begin);
   if (tid < head) f(begin + tid, as_f32(row[begin + tid]));
   const int first = begin + head;
@@ -110,24 +116,43 @@ __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
   if (tail < end) f(tail, as_f32(row[tail]));
 }
 
-// Running sums over the wave's lanes, by DPP: not through LDS.
-__device__ __forceinline__ u64 wave_run_up(u64 v) {
-#define LPX_ADD_FROM(ctrl, rows)                                                   \
-  {                                                                                \
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(                     \
-        0, (int)(unsigned)v, ctrl, rows, 0xf, false);                              \
-    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(                     \
-        0, (int)(unsigned)(v >> 32), ctrl, rows, 0xf, false);                      \
-    v += (u64)hi << 32 | lo;                                                       \
+// Over the wave's lanes by DPP, not through LDS: what a lane takes from lanes
+// below it (0 where there are none).
+#define LPX_FROM(v, ctrl, rows) \
+  (unsigned)__builtin_amdgcn_update_dpp(0, (int)(v), ctrl, rows, 0xf, false)
+#define LPX_ROW_STEPS(STEP) /* row_shr 1, 2, 4, 8: within 16 lanes */ \
+  STEP(0x111, 0xf) STEP(0x112, 0xf) STEP(0x114, 0xf) STEP(0x118, 0xf)
+#define LPX_SIX_STEPS(STEP) /* and row_bcast 15 and 31 */ \
+  LPX_ROW_STEPS(STEP) STEP(0x142, 0xa) STEP(0x143, 0xc)
+#define LPX_ADD_64(ctrl, rows)                            \
+  {                                                       \
+    const unsigned lo = LPX_FROM((unsigned)v, ctrl, rows); \
+    v += (u64)LPX_FROM(v >> 32, ctrl, rows) << 32 | lo;    \
   }
-  LPX_ADD_FROM(0x111, 0xf)  // row_shr 1, 2, 4, 8: within 16 lanes
-  LPX_ADD_FROM(0x112, 0xf)
-  LPX_ADD_FROM(0x114, 0xf)
-  LPX_ADD_FROM(0x118, 0xf)
-  LPX_ADD_FROM(0x142, 0xa)  // row_bcast 15 and 31: what stands before them
-  LPX_ADD_FROM(0x143, 0xc)
-#undef LPX_ADD_FROM
+#define LPX_ADD_32(ctrl, rows) v += LPX_FROM(v, ctrl, rows);
+#define LPX_MAX_32(ctrl, rows) v = max(v, LPX_FROM(v, ctrl, rows));
+
+// Running sums.
+__device__ __forceinline__ u64 wave_run_up(u64 v) {
+  LPX_SIX_STEPS(LPX_ADD_64)
   return v;
+}
+__device__ __forceinline__ unsigned wave_run_up(unsigned v) {
+  LPX_SIX_STEPS(LPX_ADD_32)
+  return v;
+}
+
+// Bits of 16 lanes, to the last of them.
+__device__ __forceinline__ unsigned row_or(unsigned v) {
+#define LPX_OR_32(ctrl, rows) v |= LPX_FROM(v, ctrl, rows);
+  LPX_ROW_STEPS(LPX_OR_32)
+  return v;
+}
+
+// The largest, to every lane.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+  LPX_SIX_STEPS(LPX_MAX_32)
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // ---- a row's weights and bins --------------------------------------------
@@ -392,7 +417,7 @@ __device__ __forceinline__ void run_up(ChunkBins& b, RowShared& sh) {
   unsigned c = 0;
   if (t < BINS) {
     m = wave_run_up(b.mass[t]);
-    c = (unsigned)wave_run_up((u64)b.count[t]);
+    c = wave_run_up(b.count[t]);
     if (lane == 63) {
       sh.wave_mass[t >> 6] = m;
       sh.wave_count[t >> 6] = c;
@@ -461,7 +486,7 @@ struct RowPick {
 
   // Lists the members of bins [from, to], unless a wave's are too many.
   __device__ __forceinline__ void collect(int from, int to) {
-    constexpr int VEC = 16 / sizeof(T), AHEAD = 4;
+    constexpr int VEC = LOAD<T> / sizeof(T), AHEAD = 4;
     typedef T V __attribute__((ext_vector_type(VEC)));
     // the bins as an interval, so that a logit takes two comparisons
     const float low = bin_begin(r, to);
@@ -483,7 +508,7 @@ struct RowPick {
       if (in && at < LIST) sh.list[wave][at] = order_of(x, i);
       have += __popcll(who);
     };
-    const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
+    const int off = (int)((uintptr_t)row % LOAD<T> / sizeof(T));
     const int head = min(off ? VEC - off : 0, a.vocab);
     const int vecs = (a.vocab - head) / VEC;
     const V* body = reinterpret_cast<const V*>(row + head);
@@ -738,7 +763,10 @@ __global__ __launch_bounds__(ROW_THREADS) void row_whole_kernel(SampleArgs a) {
 // negative ones their bits. Ranks below that of +inf are NaN, those from
 // that of -inf on are -inf and NaN.
 
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
 constexpr int GROUPS = 1024;  // of 64 neighbouring ranks
+constexpr unsigned MANY_COPIES = 64;  // of a value; fewer are listed
 static_assert(SAMPLE_MOST_16 == GROUPS * 512, "a row's counts of 512 logits");
 
 template <typename T> struct Ranks;
@@ -769,12 +797,17 @@ struct TableShared {
   unsigned last, lowest;   // that value's rank (0: none) and count
   u64 mass[GROUPS];        // of 64 ranks; running sums later
   unsigned members[GROUPS];  // counted for top-k; later for 512 logits each
-  u64 wave_sum[ROW_THREADS / 64], wave_sum2[ROW_THREADS / 64];
+  u64 wave_mass[ROW_THREADS / 64];
+  unsigned wave_members[ROW_THREADS / 64];
   unsigned first;          // the highest logit's rank
   unsigned logits;
   u64 minp;
   int group;
   unsigned rank, copy;     // a border's answer: its value, which of equal ones
+  unsigned listed, list[MANY_COPIES];  // those
+  int lowest_at;           // greedy: the token
+  unsigned groups;         // that hold something
+  unsigned short group_list[GROUPS];
   u64 kept;                // and the running mass with it
   int token;
 };
@@ -787,20 +820,6 @@ __device__ __forceinline__ float logit_at(unsigned rank) {
 __device__ __forceinline__ unsigned count_at(const TableShared& sh, unsigned rank) {
   if (rank == sh.last) return sh.lowest;
   return (sh.count[rank & 0x7fff] >> (rank >> 15 ? 16 : 0)) & 0xffffu;
-}
-
-// The largest of the wave's lanes.
-__device__ __forceinline__ unsigned wave_max(unsigned v) {
-#define LPX_MAX_FROM(ctrl, rows)                                                   \
-  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false));
-  LPX_MAX_FROM(0x111, 0xf)  // row_shr 1, 2, 4, 8; row_bcast 15 and 31
-  LPX_MAX_FROM(0x112, 0xf)
-  LPX_MAX_FROM(0x114, 0xf)
-  LPX_MAX_FROM(0x118, 0xf)
-  LPX_MAX_FROM(0x142, 0xa)
-  LPX_MAX_FROM(0x143, 0xc)
-#undef LPX_MAX_FROM
-  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // The value at which the running count (mass) reaches `border`, which of its
@@ -824,7 +843,7 @@ __device__ __forceinline__ void find_border(TableShared& sh, const RowScale& r,
     // before this value
     const u64 mass = (group ? sh.mass[group - 1] : 0) + wave_run_up(n * w) - n * w;
     const u64 members =
-        by_count ? (group ? sh.members[group - 1] : 0) + wave_run_up(n) - n : 0;
+        by_count ? (group ? sh.members[group - 1] : 0) + wave_run_up((unsigned)n) - n : 0;
     const u64 was = by_count ? members : mass, each = by_count ? 1 : w;
     if (was < border && was + n * each >= border) {
       // how many copies reach it: border - was of `each`, rounded up
@@ -844,27 +863,52 @@ __device__ __forceinline__ void find_border(TableShared& sh, const RowScale& r,
 }
 
 // Running sums over the workgroup's threads.
-__device__ __forceinline__ u64 block_run_up(u64 v, u64* waves) {
+template <typename N>
+__device__ __forceinline__ N block_run_up(N v, N* waves) {
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   v = wave_run_up(v);
   if (lane == 63) waves[wave] = v;
   __syncthreads();
-  const u64 up = wave_run_up(lane < ROW_THREADS / 64 ? waves[lane] : 0);
-  const u64 before = __shfl(up, max(wave - 1, 0), 64);
+  const N up = wave_run_up(lane < ROW_THREADS / 64 ? waves[lane] : (N)0);
+  const N before = __shfl(up, max(wave - 1, 0), 64);
   return wave ? v + before : v;
 }
+
+// The logits of one value among a row's words.
+struct Wanted {
+  unsigned both, keep;
+  __device__ __forceinline__ explicit Wanted(unsigned rank) {
+    const unsigned bits = rank >> 15 ? rank : 0x7fffu - rank;
+    both = bits << 16 | bits;
+    keep = bits ? 0xffffffffu : 0x7fff7fffu;  // -0 is 0
+  }
+  // 0 for a logit that is it
+  __device__ __forceinline__ u16x2 differ(int two) const {
+    return __builtin_bit_cast(u16x2, ((unsigned)two & keep) ^ both);
+  }
+  __device__ __forceinline__ bool among(i32x4 v) const {
+    const u16x2 d = __builtin_elementwise_min(
+        __builtin_elementwise_min(differ(v[0]), differ(v[1])),
+        __builtin_elementwise_min(differ(v[2]), differ(v[3])));
+    return !d[0] || !d[1];
+  }
+  __device__ __forceinline__ unsigned copies(i32x4 v) const {
+    u16x2 d = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      d += __builtin_elementwise_min(differ(v[j]), u16x2{1, 1});
+    return 8u - d[0] - d[1];
+  }
+};
 
 // The index of copy number `copy` of a value: the copies in every 512 logits
 // are counted, and those that hold the one meant looked at again.
 __device__ __forceinline__ int index_of(TableShared& sh, const unsigned short* row,
                                         int n, unsigned rank, unsigned copy) {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   const int t = (int)threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   constexpr int WAVES = ROW_THREADS / 64;
-  const unsigned bits = rank >> 15 ? rank : 0x7fffu - rank;
-  const unsigned both = bits << 16 | bits;
-  const unsigned keep = bits ? 0xffffffffu : 0x7fff7fffu;  // -0 is 0
+  const Wanted wanted(rank);
   auto load = [&](int at) {
     i32x4 v;
     if (at + 8 <= n) {
@@ -873,19 +917,10 @@ __device__ __forceinline__ int index_of(TableShared& sh, const unsigned short* r
       unsigned short w[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        w[j] = at + j < n ? row[at + j] : (unsigned short)(bits ^ 0x4000u);
+        w[j] = at + j < n ? row[at + j] : (unsigned short)(wanted.both ^ 0x4000u);
       __builtin_memcpy(&v, w, 16);
     }
     return v;
-  };
-  // 0 for a logit that is it, otherwise 1
-  auto differ = [&](int v) {
-    const u16x2 d = __builtin_bit_cast(u16x2, ((unsigned)v & keep) ^ both);
-    return __builtin_elementwise_min(d, u16x2{1, 1});
-  };
-  auto copies = [&](i32x4 v) {
-    const u16x2 d = differ(v[0]) + differ(v[1]) + differ(v[2]) + differ(v[3]);
-    return 8u - d[0] - d[1];
   };
   sh.members[t] = 0;
   __syncthreads();
@@ -898,16 +933,16 @@ __device__ __forceinline__ int index_of(TableShared& sh, const unsigned short* r
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (b + j * WAVES >= blocks) break;
-      const unsigned have = copies(v[j]);
+      const unsigned have = wanted.copies(v[j]);
       if (__ballot(have != 0)) {
-        const u64 all = wave_run_up(have);
-        if (lane == 63) sh.members[b + j * WAVES] = (unsigned)all;
+        const unsigned all = wave_run_up(have);
+        if (lane == 63) sh.members[b + j * WAVES] = all;
       }
     }
   }
   __syncthreads();
   const unsigned here = sh.members[t];
-  const unsigned through = (unsigned)block_run_up(here, sh.wave_sum);
+  const unsigned through = block_run_up(here, sh.wave_members);
   if (through - here <= copy && copy < through) {
     sh.group = t;
     sh.copy = copy - (through - here);
@@ -916,12 +951,12 @@ __device__ __forceinline__ int index_of(TableShared& sh, const unsigned short* r
   if (wave == 0) {
     const int at = sh.group * 512 + lane * 8;
     const i32x4 v = load(at);
-    const unsigned have = copies(v), up = (unsigned)wave_run_up(have);
+    const unsigned have = wanted.copies(v), up = wave_run_up(have);
     unsigned left = sh.copy - (up - have);
     if (up - have <= sh.copy && sh.copy < up) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const u16x2 d = differ(v[j / 2]);
+        const u16x2 d = wanted.differ(v[j / 2]);
         if (!d[j % 2] && left-- == 0) sh.token = at + j;
       }
     }
@@ -943,6 +978,28 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   const unsigned short* x = static_cast<const unsigned short*>(a.logits) + row * a.stride;
   const bool greedy = !(param(a.temperature, row) > 0);
 
+  // The row: 16-B vectors, STEP at a time, and the elements at its ends, one
+  // for each of 16 threads. The first loads go out before all else, and the
+  // last ones' registers are kept for the search for the index.
+  constexpr int AHEAD = 4, STEP = AHEAD * ROW_THREADS;
+  const int vocab = a.vocab;
+  const int off = (int)(((uintptr_t)x & 15) / 2);
+  const int head = min(off ? 8 - off : 0, vocab);
+  const int vecs = (vocab - head) / 8;
+  const i32x4* body = reinterpret_cast<const i32x4*>(x + head);
+  auto load = [&](i32x4* to, int first) {
+#pragma unroll
+    for (int l = 0; l < AHEAD; ++l)
+      if (first + l * ROW_THREADS < vecs)
+        to[l] = body[min(first + l * ROW_THREADS + lane, vecs - 1)];
+  };
+  int v0 = wave * 64;
+  i32x4 v[AHEAD];
+  load(v, v0);
+  int edge = vocab;
+  if (t < 16) edge = t < 8 ? (t < head ? t : vocab) : head + vecs * 8 + t - 8;
+  const unsigned edge_bits = edge < vocab ? x[edge] : 0u;
+
   {
     const i32x4 zero = {0, 0, 0, 0};
     i32x4* words = reinterpret_cast<i32x4*>(sh.count);
@@ -961,12 +1018,14 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
       sh.copy = 0;
       sh.kept = 0;
       sh.token = -1;
+      sh.listed = 0;
+      sh.groups = 0;
+      sh.lowest_at = 0x7fffffff;
     }
   }
   __syncthreads();
 
   // Counts, and the highest: of ranks from +inf's on, of which NaN's are not.
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   u16x2 lows = {0xffff, 0xffff};
   auto highest = [&](unsigned two) {
     const u16x2 above = __builtin_bit_cast(u16x2, two) -
@@ -980,70 +1039,68 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   // by them. So where the lowest of the 2048 logits that a wave holds is in
   // many of its lanes, they count it in a register.
   unsigned last = 0, lowest = 0;
-  constexpr int AHEAD = 4, MANY_LANES = 8;
-  const int vocab = a.vocab;
-  const int off = (int)(((uintptr_t)x & 15) / 2);
-  const int head = min(off ? 8 - off : 0, vocab);
-  const int vecs = (vocab - head) / 8;
-  const i32x4* body = reinterpret_cast<const i32x4*>(x + head);
-  if (t < 16) {  // the ends
-    const int at = t < 8 ? t : head + vecs * 8 + t - 8;
-    if (at < (t < 8 ? head : vocab)) {
-      const unsigned two = ranks_of((unsigned)x[at] * 0x10001u);
-      highest(two);
-      if (!greedy) add(two & 0xffffu, 1u);
-    }
-  }
-  for (int v0 = wave * 64; v0 < vecs; v0 += AHEAD * ROW_THREADS) {
-    i32x4 v[AHEAD];
-#pragma unroll
-    for (int l = 0; l < AHEAD; ++l)
-      if (v0 + l * ROW_THREADS < vecs)
-        v[l] = body[min(v0 + l * ROW_THREADS + lane, vecs - 1)];
+  constexpr int MANY_LANES = 8;
+  if (!greedy && edge < vocab) add(ranks_of(edge_bits) & 0xffffu, 1u);
+  unsigned best = 0xffffu;  // greedy: the lane's highest, and where it came first
+  int best_at = 0;
+  while (v0 < vecs) {
+    const bool more = v0 + STEP < vecs;
+    i32x4 next[AHEAD];
+    if (more) load(next, v0 + STEP);
     u16x2 most = {0, 0};
 #pragma unroll
     for (int l = 0; l < AHEAD; ++l) {
       if (v0 + l * ROW_THREADS >= vecs) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v[l][j] = (int)ranks_of((unsigned)v[l][j]);
-        highest((unsigned)v[l][j]);
-        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[l][j]));
+        const unsigned two = ranks_of((unsigned)v[l][j]);
+        highest(two);
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, two));
       }
     }
-    if (greedy) continue;
-    const unsigned own = min(max((unsigned)most[0], (unsigned)most[1]), Ranks<T>::NONE);
-    const unsigned far = wave_max(own);
-    const bool often = far >= last && __popcll(__ballot(own == far)) >= MANY_LANES;
-    if (often && far > last) {
-      if (lowest) add(last, lowest);
-      last = far;
-      lowest = 0;
-    }
+    if (greedy) {
+      const unsigned now = min(lows[0], lows[1]);
+      if (now < best) {
+        best = now;
+        best_at = v0;
+      }
+    } else {
+      const unsigned own = min(max((unsigned)most[0], (unsigned)most[1]), Ranks<T>::NONE);
+      const unsigned far = wave_max(own);
+      const bool often = far >= last && __popcll(__ballot(own == far)) >= MANY_LANES;
+      if (often && far > last) {
+        if (lowest) add(last, lowest);
+        last = far;
+        lowest = 0;
+      }
 #pragma unroll
-    for (int l = 0; l < AHEAD; ++l) {
-      const int at = v0 + l * ROW_THREADS;
-      if (at >= vecs) break;
-      if (at + lane >= vecs) continue;
-      if (often) {
+      for (int l = 0; l < AHEAD; ++l) {
+        const int at = v0 + l * ROW_THREADS;
+        if (at >= vecs) break;
+        if (at + lane >= vecs) continue;
+        if (often) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const unsigned rank = (unsigned)v[l][j / 2] >> (j % 2 * 16) & 0xffffu;
-          if (rank == last)
-            ++lowest;
-          else
-            add(rank, 1u);
+          for (int j = 0; j < 8; ++j) {
+            const unsigned rank = ranks_of((unsigned)v[l][j / 2]) >> (j % 2 * 16) & 0xffffu;
+            if (rank == last)
+              ++lowest;
+            else
+              add(rank, 1u);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            add(ranks_of((unsigned)v[l][j / 2]) >> (j % 2 * 16) & 0xffffu, 1u);
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          add((unsigned)v[l][j / 2] >> (j % 2 * 16) & 0xffffu, 1u);
       }
     }
-  }
-  unsigned low = min((unsigned)lows[0], (unsigned)lows[1]);
+    if (!more) break;
 #pragma unroll
-  for (int m = 32; m > 0; m >>= 1) low = min(low, (unsigned)__shfl_xor(low, m, 64));
+    for (int l = 0; l < AHEAD; ++l) v[l] = next[l];
+    v0 += STEP;
+  }
+  if (edge < vocab) highest(ranks_of(edge_bits * 0x10001u));
+  const unsigned low = 0xffffu - wave_max(0xffffu - min(lows[0], lows[1]));
   if (lane == 0) {
     atomicMin(&sh.first, low);
     atomicMax(&sh.last, last);
@@ -1056,12 +1113,33 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   }
   if (first == 0x8000u) first = 0x7fffu;
   if (greedy) {
-    const int token = index_of(sh, x, a.vocab, first, 0);
+    int token;
+    if (first == 0x7fffu) {  // +0 and -0 are one
+      token = index_of(sh, x, vocab, first, 0);
+    } else {
+      const Wanted wanted(first);
+      int at = vocab;
+      if (edge < vocab && !wanted.differ((int)edge_bits)[0]) at = edge;
+      if (best == first - Ranks<T>::INF) {
+        load(v, best_at);
+#pragma unroll
+        for (int l = AHEAD - 1; l >= 0; --l) {
+          const int i = best_at + l * ROW_THREADS + lane;
+          if (i >= vecs || !wanted.among(v[l])) continue;
+#pragma unroll
+          for (int j = 7; j >= 0; --j)
+            if (!wanted.differ(v[l][j / 2])[j % 2]) at = min(at, head + i * 8 + j);
+        }
+      }
+      if (at < vocab) atomicMin(&sh.lowest_at, at);
+      __syncthreads();
+      token = sh.lowest_at;
+    }
     if (t == 0) a.token[row] = token;
     return;
   }
   {
-    const unsigned n = (unsigned)wave_run_up((u64)lowest);
+    const unsigned n = wave_run_up(lowest);
     if (lane == 63 && n) {
       if (last == sh.last)
         atomicAdd(&sh.lowest, n);
@@ -1085,7 +1163,6 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
     const unsigned at = sh.last & 0x7fff, half = sh.last >> 15 << 4;
     sh.lowest += sh.count[at] >> half & 0xffffu;
     sh.count[at] = (sh.count[at] & ~(0xffffu << half)) | 1u << half;
-    sh.logits = sh.lowest - 1u;
   }
   __syncthreads();
 
@@ -1094,44 +1171,44 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   e.at = 0;
   const RowScale r = row_scale(a, row, e);
   const u64 least = least_weight(a, row, r);
-  // Sums of groups of 64 ranks. Most words hold nothing: a wave looks at 256
-  // of them at once, and at the groups of those that do one by one.
-  u64 minp = 0;
-  unsigned all = 0;
-  for (int b = wave; b < 128; b += ROW_THREADS / 64) {
-    const i32x4 v = *reinterpret_cast<const i32x4*>(sh.count + b * 256 + lane * 4);
+  // Sums of groups of 64 ranks. A list of those that hold something, of which
+  // each wave takes its share: weights are most of the work.
+  constexpr int WAVES = ROW_THREADS / 64;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) all += ((unsigned)v[j] & 0xffffu) + ((unsigned)v[j] >> 16);
-    if (!__ballot((v[0] | v[1] | v[2] | v[3]) != 0)) continue;
-    unsigned two[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) two[j] = sh.count[b * 256 + j * 64 + lane];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int group = b * 4 + (j & 3) + (j >> 2) * (GROUPS / 2);
-      const unsigned rank = (unsigned)group * 64 + lane;
-      unsigned n = j >> 2 ? two[j & 3] >> 16 : two[j & 3] & 0xffffu;
-      if (rank == sh.last) n = sh.lowest;
-      if (rank < Ranks<T>::INF || rank >= Ranks<T>::NONE) n = 0;
-      if (!__ballot(n != 0)) continue;
-      const u64 w = weight(r, logit_at<T>(rank));
-      u64 mass = n * w;
-      if (w >= least) minp += mass;
-      mass = wave_run_up(mass);
-      unsigned members = 0;
-      if (r.by_k) members = (unsigned)wave_run_up((u64)n);
-      if (lane == 63) {
-        sh.mass[group] = mass;
-        sh.members[group] = members;
-      }
+  for (int i = 0; i < 128 / WAVES; ++i) {
+    const int b = i * WAVES + wave;  // 16 lanes read 64 words
+    const i32x4 c = *reinterpret_cast<const i32x4*>(sh.count + b * 256 + lane * 4);
+    const unsigned some = row_or((unsigned)(c[0] | c[1] | c[2] | c[3]));
+    if ((lane & 15) == 15 && some) {
+      const int group = b * 4 + lane / 16;
+      if (some & 0xffffu) sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)group;
+      if (some >> 16)
+        sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)(group + GROUPS / 2);
     }
   }
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) {
-    all += __shfl_xor(all, m, 64);
-    minp += __shfl_xor(minp, m, 64);
+  __syncthreads();
+  u64 minp = 0;
+  unsigned all = 0;
+  const int groups = (int)sh.groups, share = (groups + WAVES - 1) / WAVES;
+  for (int i = wave * share; i < min(groups, wave * share + share); ++i) {
+    const int group = __builtin_amdgcn_readfirstlane(sh.group_list[i]);
+    const unsigned rank = (unsigned)group * 64 + lane;
+    unsigned n = count_at(sh, rank);
+    all += n;
+    if (rank < Ranks<T>::INF || rank >= Ranks<T>::NONE) n = 0;
+    const u64 w = weight(r, logit_at<T>(rank));
+    u64 mass = n * w;
+    if (w >= least) minp += mass;
+    mass = wave_run_up(mass);
+    if (r.by_k) n = wave_run_up(n);
+    if (lane == 63) {
+      sh.mass[group] = mass;
+      sh.members[group] = n;
+    }
   }
-  if (lane == 0) {
+  all = wave_run_up(all);
+  minp = wave_run_up(minp);
+  if (lane == 63) {
     atomicAdd(&sh.logits, all);
     atomicAdd(&sh.minp, minp);
   }
@@ -1143,10 +1220,10 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   }
   // Running sums; thread t has group t
   {
-    const u64 m = block_run_up(sh.mass[t], sh.wave_sum);
-    const u64 n = r.by_k ? block_run_up(sh.members[t], sh.wave_sum2) : 0;
+    const u64 m = block_run_up(sh.mass[t], sh.wave_mass);
+    const unsigned n = r.by_k ? block_run_up(sh.members[t], sh.wave_members) : 0;
     sh.mass[t] = m;
-    sh.members[t] = (unsigned)n;
+    sh.members[t] = n;
   }
   __syncthreads();
 
@@ -1162,8 +1239,44 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   }
   kept = min(kept, sh.minp);
   find_border<T>(sh, r, false, draw_border(param(a.u, row), kept));
-  const int token = index_of(sh, x, a.vocab, sh.rank, sh.copy);
-  if (t == 0) a.token[row] = token;
+  const unsigned rank = sh.rank;
+  const unsigned copies = count_at(sh, rank);
+  if (copies > MANY_COPIES) {
+    const int token = index_of(sh, x, vocab, rank, sh.copy);
+    if (t == 0) a.token[row] = token;
+    return;
+  }
+  // A few copies: their indices to a list, from the last loads back to the
+  // first; the answer has `copy` of them below it.
+  const Wanted wanted(rank);
+  auto list = [&](int at) {
+    const unsigned i = atomicAdd(&sh.listed, 1u);
+    if (i < MANY_COPIES) sh.list[i] = (unsigned)at;
+  };
+  if (edge < vocab && !wanted.differ((int)edge_bits)[0]) list(edge);
+  if (v0 >= vecs) v0 -= STEP;  // a wave without vectors
+  while (v0 >= 0) {
+    i32x4 next[AHEAD];
+    if (v0 >= STEP) load(next, v0 - STEP);
+#pragma unroll
+    for (int l = 0; l < AHEAD; ++l) {
+      const int at = v0 + l * ROW_THREADS + lane;
+      if (at >= vecs || !wanted.among(v[l])) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (!wanted.differ(v[l][j / 2])[j % 2]) list(head + at * 8 + j);
+    }
+    v0 -= STEP;
+#pragma unroll
+    for (int l = 0; l < AHEAD; ++l) v[l] = next[l];
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const unsigned listed = min(sh.listed, MANY_COPIES);
+  const unsigned own = sh.list[min((unsigned)lane, MANY_COPIES - 1)];
+  unsigned below = 0;
+  for (unsigned i = 0; i < listed; ++i) below += sh.list[i] < own;
+  if ((unsigned)lane < listed && below == sh.copy) a.token[row] = own;
 }
 
 template <typename T>

@@ -911,3 +911,23 @@ def test_sample_rows_that_are_mostly_masked(dtype, mask, settings):
     x[5] = torch.where(there[5] < 0.6, m, -m if mask == 0.0 else x[5])
     u = _uniform(6, 87)
     _same_tokens(ops.sample(x, u, **settings), x, u, **settings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [1, 7, 9, 8191, 32773, 65543, 140009])
+def test_sample_greedy_takes_the_first_of_the_highest(dtype, v):
+    # rows that begin at every offset from a 16-byte boundary
+    buf = _randn((9, v + 9), 88, dtype)
+    x = torch.as_strided(buf, (8, v), (v + 10, 1), 1)
+    top = x.float().max().item() * 2 + 1
+    for i in range(8):
+        for at in ((i * 131) % v, v // 2, v - 1, (i * 7919 + 5) % v):
+            x[i, at] = top
+    x[6] = 0.0
+    x[6, 3::5] = -0.0
+    x[7] = -0.0
+    if v > 9:
+        x[7, 9:] = 0.0
+    want = [(r == r.max()).nonzero()[0].item() for r in x.cpu().float()]
+    assert ops.sample(x, _uniform(8, 89), temperature=0.0).tolist() == want
