@@ -128,13 +128,6 @@ def matmul_mx_w4(A: torch.Tensor, B: torch.Tensor) -> torch.Tensor:
 
 # ---- decode-step operators on quantised weights ---------------------------
 
-def _inference_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under "
-                           "torch.no_grad() or on detached tensors")
-
-
 def rmsnorm(x: torch.Tensor, weight: torch.Tensor,
             residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """Root-mean-square norm over the last axis, of x or of x + residual.
@@ -143,9 +136,7 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor,
     unrounded h, rounded once. x [..., K] bf16/fp16/f32 (rows may be strided),
     residual like x, weight [K] of x's type or f32. Returns y, or (y, h) if a
     residual is given: h, rounded to x's type, is the next layer's residual."""
-    _inference_only("rmsnorm", x, weight, residual)
-    out = require_extension().rmsnorm(x, weight, residual, eps)
-    return out[0] if residual is None else tuple(out)
+    return require_extension().rmsnorm(x, weight, residual, eps)
 
 
 def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor,
@@ -158,8 +149,7 @@ def rmsnorm_mx(x: torch.Tensor, weight: torch.Tensor,
     scale is the smallest power of two that brings its largest to 448 at most
     (2^0 for a block of zeros and for the blocks that pad the last scale
     tile); NaN and infinities become the payload's NaN."""
-    _inference_only("rmsnorm_mx", x, weight, residual)
-    return tuple(require_extension().rmsnorm_mx(x, weight, residual, eps))
+    return require_extension().rmsnorm_mx(x, weight, residual, eps)
 
 
 def gemv_w4(x: torch.Tensor, Bt4: torch.Tensor, sB: torch.Tensor,
@@ -171,7 +161,6 @@ def gemv_w4(x: torch.Tensor, Bt4: torch.Tensor, sB: torch.Tensor,
     quantize_mx_fp4, any N, K%64==0. Returns [..., N] f32, or bf16. Made for
     one to 64 rows, where reading the weights is all the time; more rows are
     taken 64 at a time. Sums in f32, in a fixed order."""
-    _inference_only("gemv_w4", x)
     return require_extension().gemv_w4(x, Bt4, sB, bf16_out)
 
 

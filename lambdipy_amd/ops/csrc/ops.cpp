@@ -793,6 +793,11 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& l
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
+void inference_only(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
+              " has no backward pass: call it under torch.no_grad() or on detached tensors");
+}
+
 // Rows of a 2-D view whose last axis is dense; rows may be further apart.
 at::Tensor dense_rows(const at::Tensor& t) {
   const at::Tensor v = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -808,6 +813,9 @@ struct NormCall {
 NormCall norm_call(const at::Tensor& x, const at::Tensor& weight,
                    const std::optional<at::Tensor>& residual, double eps,
                    const char* what) {
+  inference_only(x, what);
+  inference_only(weight, what);
+  if (residual.has_value()) inference_only(*residual, what);
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, " expects x [..., K], K >= 1");
   const int64_t K = x.size(-1);
   NormCall c;
@@ -836,8 +844,8 @@ NormCall norm_call(const at::Tensor& x, const at::Tensor& weight,
   return c;
 }
 
-std::vector<at::Tensor> rmsnorm(const at::Tensor& x, const at::Tensor& weight,
-                                const std::optional<at::Tensor>& residual, double eps) {
+py::object rmsnorm(const at::Tensor& x, const at::Tensor& weight,
+                   const std::optional<at::Tensor>& residual, double eps) {
   NormCall c = norm_call(x, weight, residual, eps, "rmsnorm");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
   auto y = fresh(x.sizes(), x.scalar_type(), x);
@@ -848,12 +856,12 @@ std::vector<at::Tensor> rmsnorm(const at::Tensor& x, const at::Tensor& weight,
                          c.r.defined() ? c.h.data_ptr() : nullptr, y.data_ptr(),
                          c.R, c.K, current_stream(x)),
             "rmsnorm");
-  if (c.r.defined()) return {y, c.h};
-  return {y};
+  if (c.r.defined()) return py::make_tuple(y, c.h);
+  return py::cast(y);
 }
 
-std::vector<at::Tensor> rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight,
-                                   const std::optional<at::Tensor>& residual, double eps) {
+py::object rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight,
+                      const std::optional<at::Tensor>& residual, double eps) {
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 64 == 0, "rmsnorm_mx expects x [..., K%64==0]");
   NormCall c = norm_call(x, weight, residual, eps, "rmsnorm_mx");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -867,8 +875,8 @@ std::vector<at::Tensor> rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight
                             q.data_ptr<uint8_t>(), sc.data_ptr<uint8_t>(), c.R, c.K,
                             current_stream(x)),
             "rmsnorm_mx");
-  if (c.r.defined()) return {q, sc, c.h};
-  return {q, sc};
+  if (c.r.defined()) return py::make_tuple(q, sc, c.h);
+  return py::make_tuple(q, sc);
 }
 
 // Weights as quantize_mx4 gives them: [N, K/2] and [ceil(K/128), N, 4].
@@ -886,6 +894,7 @@ void check_w4(const at::Tensor& w, const at::Tensor& sw, int64_t K, const char* 
 
 at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor& sB,
                    bool bf16_out) {
+  inference_only(x, "gemv_w4");
   TORCH_CHECK(x.dim() >= 1, "gemv_w4 expects x [..., K]");
   TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf,
               "gemv_w4 supports bf16 and fp16 activations, got ", x.scalar_type());

@@ -1289,7 +1289,9 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   } else {
     const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
     chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
-    chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+    const SampleParam& t = a.temperature;
+    if (t.kind != SampleParam::value_ || t.value > 0)  // not known to be greedy
+      chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
     row_pick_kernel<T><<<rows, threads, 0, stream>>>(a);
   }
   return hipGetLastError();
