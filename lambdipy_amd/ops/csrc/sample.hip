@@ -214,10 +214,13 @@ __device__ __forceinline__ RowScale row_scale(const SampleArgs& a, int row,
 }
 
 // The row's extent from its chunks': every wave works it out for itself.
-__device__ __forceinline__ Extent row_extent(const SampleArgs& a, int row) {
+// `own`: the lane's, or the last.
+__device__ __forceinline__ Extent row_extent(const SampleArgs& a, int row,
+                                             ChunkMax own) {
   const ChunkMax* c = a.maxima + (long)row * a.chunks;
   Extent e;
-  for (int i = (int)threadIdx.x & 63; i < a.chunks; i += 64)
+  e.join(own.hi, own.lo, own.at);
+  for (int i = 64 + ((int)threadIdx.x & 63); i < a.chunks; i += 64)
     e.join(c[i].hi, c[i].lo, c[i].at);
   e.join_wave();
   return e;
@@ -335,7 +338,9 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a)
   const int row = (int)blockIdx.x / a.chunks;
   const int begin = (int)blockIdx.x % a.chunks * a.chunk;
   const int end = min(begin + a.chunk, a.vocab);
-  const RowScale r = row_scale(a, row, row_extent(a, row));
+  const ChunkMax* maxima = a.maxima + (long)row * a.chunks;
+  const ChunkMax own = maxima[min((int)threadIdx.x & 63, a.chunks - 1)];
+  const RowScale r = row_scale(a, row, row_extent(a, row, own));
   if (r.greedy) return;
   __shared__ ChunkBins b;
   b.mass[threadIdx.x] = 0;
@@ -371,7 +376,7 @@ __device__ __forceinline__ float bin_begin(const RowScale& r, int bin) {
   const auto up = [](float x) { return ~(unsigned)(order_of(x, 0) >> 32); };
   const unsigned most = up(r.hi), least = up(-3.402823466e38f);
   unsigned at = 0;
-#pragma unroll
+#pragma unroll 1
   for (int shift = 26; shift >= -4; shift -= 6) {
     const int s = max(shift, 0);
     const unsigned lane = threadIdx.x & 63;
@@ -496,17 +501,16 @@ struct RowPick {
     const int lane = (int)threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     // Each wave has a list of its own and knows its length: no atomic, whose
-    // answer would have to be waited for. All lanes come here together.
+    // answer would have to be waited for. First of indices: a lane has a bit
+    // for each of its logits.
     int have = 0;
-    auto add = [&](bool there, int i, float x) {
-      const bool in = there && low <= x && x <= high;
-      const u64 who = __ballot(in);
-      if (!who) return;
-      const int at = have + (int)__builtin_amdgcn_mbcnt_hi(
-                                (unsigned)(who >> 32),
-                                __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
-      if (in && at < LIST) sh.list[wave][at] = order_of(x, i);
-      have += __popcll(who);
+    u64* list = sh.list[wave];
+    auto in = [&](float x) { return __builtin_amdgcn_fmed3f(x, low, high) == x; };
+    auto add = [&](unsigned bits, auto index) {
+      const unsigned n = (unsigned)__popc(bits), up = wave_run_up(n);
+      for (unsigned at = have + up - n; bits; bits &= bits - 1, ++at)
+        if (at < LIST) list[at] = (unsigned)index(__builtin_ctz(bits));
+      have += __builtin_amdgcn_readlane((int)up, 63);
     };
     const int off = (int)((uintptr_t)row % LOAD<T> / sizeof(T));
     const int head = min(off ? VEC - off : 0, a.vocab);
@@ -514,22 +518,36 @@ struct RowPick {
     const V* body = reinterpret_cast<const V*>(row + head);
     if (wave == 0) {
       const int tail = head + vecs * VEC + lane;
-      add(lane < head, lane, lane < head ? as_f32(row[lane]) : 0.f);
-      add(tail < a.vocab, tail, tail < a.vocab ? as_f32(row[tail]) : 0.f);
+      const unsigned first = lane < head && in(as_f32(row[lane]));
+      const unsigned last = tail < a.vocab && in(as_f32(row[tail]));
+      add(first | last << 1, [&](int bit) { return bit ? tail : lane; });
     }
     for (int v0 = wave * 64; v0 < vecs; v0 += AHEAD * ROW_THREADS) {
       V v[AHEAD];
 #pragma unroll
       for (int l = 0; l < AHEAD; ++l)
         v[l] = body[min(v0 + l * ROW_THREADS + lane, vecs - 1)];
-      const bool all = v0 + (AHEAD - 1) * ROW_THREADS + 64 <= vecs;
+      unsigned bits = 0;
 #pragma unroll
-      for (int l = 0; l < AHEAD; ++l) {
-        const int at = v0 + l * ROW_THREADS + lane;
+      for (int l = 0; l < AHEAD; ++l)
 #pragma unroll
         for (int j = 0; j < VEC; ++j)
-          add(all || at < vecs, head + at * VEC + j, as_f32(v[l][j]));
+          bits |= (unsigned)in(as_f32(v[l][j])) << (l * VEC + j);
+      // those behind the row's end
+      const int left = vecs - v0 - lane;
+      if (left <= (AHEAD - 1) * ROW_THREADS) {
+        const int whole = left <= 0 ? 0 : (left + ROW_THREADS - 1) / ROW_THREADS;
+        bits &= (1u << (whole * VEC)) - 1;
       }
+      if (__ballot(bits != 0))
+        add(bits, [&](int bit) {
+          return head + (v0 + bit / VEC * ROW_THREADS + lane) * VEC + bit % VEC;
+        });
+    }
+    // then of places in the order
+    for (int i = lane; i < min(have, LIST); i += 64) {
+      const int at = (int)list[i];
+      list[i] = order_of(as_f32(row[at]), at);
     }
     if (lane == 0) sh.listed[wave] = have;
     __syncthreads();
@@ -678,6 +696,8 @@ template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   __shared__ RowShared sh;
   const int row = (int)blockIdx.x, t = (int)threadIdx.x;
+  const ChunkMax* maxima = a.maxima + (long)row * a.chunks;
+  const ChunkMax own = maxima[min(t & 63, a.chunks - 1)];
   // thread t sums bin t % BINS over a quarter of the chunks
   const ChunkBins* c = a.bins + (long)row * a.chunks;
   const int bin = t % BINS;
@@ -702,7 +722,7 @@ __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
     }
   }
   clear(sh.row);
-  const RowScale r = row_scale(a, row, row_extent(a, row));
+  const RowScale r = row_scale(a, row, row_extent(a, row, own));
   if (r.greedy) {
     if (t == 0) a.token[row] = r.at;
     return;
