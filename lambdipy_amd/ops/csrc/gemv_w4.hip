@@ -18,9 +18,10 @@
 // bytes of a row, and join their sums in LDS in a fixed order.
 //
 // Measured: 100000 x 8192 by one bf16 row 73 us, 5.9 TB/s (reading alone
-// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.4 us; 28000 x 8192 by 64
-// MX rows 44 us, where the MFMA (27% busy), the conversions to bf16, LDS and the
-// load path take about a quarter of the time each, one after another.
+// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.1 us; 28000 x 8192 by 64
+// MX rows 35 us, of which the MFMA is busy 12 and the conversions to bf16, LDS
+// and the load path about as long each; 437 tiles on 256 CUs leave a seventh
+// of them idle.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -269,33 +270,30 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
   };
 
   auto multiply = [&](Turned& q) {
-    // 16-bit weights, once for all rows of x
-    i32x4 b[NT][4];
+    if constexpr (MODE == X_F16) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if constexpr (MODE == X_F16) q.w[t] = transpose_groups(q.w[t]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        b[t][j] = MODE == X_F16
-                      ? __builtin_bit_cast(i32x4, w_f16(q.w[t][j]))
-                      : __builtin_bit_cast(i32x4, w_bf16(q.w[t][j], scale_of(q.sw[t], g)));
+      for (int t = 0; t < NT; ++t) q.w[t] = transpose_groups(q.w[t]);
     }
+    // A quarter of the step at a time, so that the next quarter's conversions
+    // go on beside this one's MFMAs.
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      i32x4 x[4];
-      if constexpr (MODE == X_MX) {
-        const i32x4 lo = q.x[i][0], hi = q.x[i][1];
-        const float sx = scale_of(q.sx[i], g);
-        x[0] = __builtin_bit_cast(i32x4, x_bf16(lo[0], lo[1], sx));
-        x[1] = __builtin_bit_cast(i32x4, x_bf16(lo[2], lo[3], sx));
-        x[2] = __builtin_bit_cast(i32x4, x_bf16(hi[0], hi[1], sx));
-        x[3] = __builtin_bit_cast(i32x4, x_bf16(hi[2], hi[3], sx));
-      } else {
+    for (int j = 0; j < 4; ++j) {
+      i32x4 b[NT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = q.x[i][j];
-      }
+      for (int t = 0; t < NT; ++t)
+        b[t] = MODE == X_F16
+                   ? __builtin_bit_cast(i32x4, w_f16(q.w[t][j]))
+                   : __builtin_bit_cast(i32x4, w_bf16(q.w[t][j], scale_of(q.sw[t], g)));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int i = 0; i < MT; ++i) {
+        i32x4 x;
+        if constexpr (MODE == X_MX) {
+          const i32x4 v = q.x[i][j / 2];
+          x = __builtin_bit_cast(
+              i32x4, x_bf16(v[j % 2 * 2], v[j % 2 * 2 + 1], scale_of(q.sx[i], g)));
+        } else {
+          x = q.x[i][j];
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           if constexpr (MODE == X_F16) {
@@ -303,7 +301,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
             // one block (its words spread over the lane groups) and the
             // block's scale goes onto the sum
             const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                __builtin_bit_cast(nf16x8, x[j]), __builtin_bit_cast(nf16x8, b[t][j]),
+                __builtin_bit_cast(nf16x8, x), __builtin_bit_cast(nf16x8, b[t]),
                 f32x4{0, 0, 0, 0}, 0, 0, 0);
             const float sc = scale_of(q.sw[t], j);
 #pragma unroll
@@ -312,13 +310,20 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
           } else {
             // MFMA j takes elements [8j, 8j+8) of the four groups' blocks
             acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                __builtin_bit_cast(nbf16x8, x[j]), __builtin_bit_cast(nbf16x8, b[t][j]),
+                __builtin_bit_cast(nbf16x8, x), __builtin_bit_cast(nbf16x8, b[t]),
                 acc[i][t], 0, 0, 0);
           }
         }
       }
     }
   };
+
+  // The next step's loads stay in front of a step's products: left to itself
+  // the compiler puts them behind, which saves registers and costs 28000 x
+  // 8192 by 64 MX rows 39 us, from 36. Other instructions may pass (0x78f:
+  // all but vector memory's) except where that is slower (8192 x 8192 by 32
+  // MX rows 9.4 us, from 8.9; by 64, tiles of 2 x 4, 12.0, and without 12.9).
+  constexpr int MAY_PASS = MODE == X_MX && MT == NT ? 0 : 0x78f;
 
   S f[DEPTH];
 #pragma unroll
@@ -330,6 +335,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
       Turned q;
       turn_round(f[d], q, turn + d);
       load(f[d], turn + d + DEPTH);  // on its way while this one is multiplied
+      __builtin_amdgcn_sched_barrier(MAY_PASS);
       multiply(q);
     }
   }
@@ -377,29 +383,39 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// The largest tile whose workgroups still fill the chip: a wave loads x once
-// for all the weight rows of its tile, so that wide tiles cost less a weight,
-// but with fewer than one workgroup a CU the rest of the chip is idle. Over
-// M = 12 .. 64 and N x K from 1000 x 2048 to 100000 x 8192 this is the
-// fastest of the sixteen shapes tried or within a tenth of it (8192 x 8192,
-// M = 64 MX: 32 x 64 tiles on 256 workgroups 12.7 us, 64 x 64 on 128 18.0;
-// 28000 x 8192: 55 and 44 us).
+// The largest tile of which more than half of the CUs get one: a wave loads
+// and converts x once for all the weight rows of its tile, so that wide tiles
+// cost less a weight, but half as wide ones on twice the CUs take less time.
+// Up to a tile a CU its waves split K eight ways; with more, four ways, and
+// two tiles share a CU. K = 8192, us:
+//   64 MX rows: N = 5500 2x4 tiles 12.3, 2x2 15.0; 8192 2x4 12.3, 4x4 18.6;
+//     9000 4x4 18.3, 2x4 23.9; 18000 4x4 by four waves 31.5, by eight 34.3
+//   32: 4096 (K too) 1x2 4.5, 2x2 5.5; 8192 2x2 8.9, 2x4 12.0; 10000 2x4
+//     12.4, 2x2 14.8; 18000 bf16 2x4 by four waves 23.5, by eight 26.5
+//   16: 8192 1x2 8.1, 1x4 9.3; 10000 1x4 9.9, 1x2 11.7
 template <int MODE>
 hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
   if (a.K < 64 || a.K % 64 != 0 || a.K > (1 << 24)) return hipErrorInvalidValue;
   constexpr long CUS = 256;
-  auto fills = [&](int mt, int nt) {
-    return (long)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt)) >= CUS;
+  auto tiles = [&](int mt, int nt) {
+    return (long)((a.M + 16 * mt - 1) / (16 * mt)) * ((a.N + 16 * nt - 1) / (16 * nt));
   };
+  auto fills = [&](int mt, int nt) { return tiles(mt, nt) > CUS / 2; };
   // Rows that one load of x holds: 100000 x 8192 by one bf16 row 73 us,
   // loading a tile of 16 rows of x 80 us.
   if (a.M <= (MODE == X_MX ? 8 : 4))
     return fills(1, 2) ? launch<MODE, 1, 2, 8, 2, true>(a, stream)
                        : launch<MODE, 1, 1, 8, 2, true>(a, stream);
   if constexpr (MODE != X_F16)  // whose scaled sums do not fit the registers
-    if (a.M > 32 && fills(4, 4)) return launch<MODE, 4, 4, 4, 1>(a, stream);
-  if (a.M > 16 && fills(2, 4)) return launch<MODE, 2, 4, 8, 1>(a, stream);
+    if (a.M > 32 && fills(4, 4))
+      return tiles(4, 4) > CUS ? launch<MODE, 4, 4, 4, 1>(a, stream)
+                               : launch<MODE, 4, 4, 8, 1>(a, stream);
+  if (a.M > 16 && fills(2, 4)) {
+    if constexpr (MODE != X_F16)  // 28000 x 8192 by 64: 72.9 us, by eight 66.8
+      if (tiles(2, 4) > CUS) return launch<MODE, 2, 4, 4, 1>(a, stream);
+    return launch<MODE, 2, 4, 8, 1>(a, stream);
+  }
   if (a.M > 16 && fills(2, 2)) return launch<MODE, 2, 2, 8, 1>(a, stream);
   if (fills(1, 4)) return launch<MODE, 1, 4, 8, 1>(a, stream);
   if (fills(1, 2)) return launch<MODE, 1, 2, 8, 1>(a, stream);
