@@ -18,10 +18,10 @@
 // bytes of a row, and join their sums in LDS in a fixed order.
 //
 // Measured: 100000 x 8192 by one bf16 row 73 us, 5.9 TB/s (reading alone
-// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.1 us; 28000 x 8192 by 64
-// MX rows 35 us, of which the MFMA is busy 12 and the conversions to bf16, LDS
-// and the load path about as long each; 437 tiles on 256 CUs leave a seventh
-// of them idle.
+// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.1 us (10.0 where all of it
+// comes from memory); 28000 x 8192 by 64 MX rows 35 and 44 us, of which the
+// MFMA is busy 12 and the conversions to bf16, LDS and the load path about as
+// long each; 437 tiles on 256 CUs leave a seventh of them idle.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -318,12 +318,10 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
     }
   };
 
-  // The next step's loads stay in front of a step's products: left to itself
-  // the compiler puts them behind, which saves registers and costs 28000 x
-  // 8192 by 64 MX rows 39 us, from 36. Other instructions may pass (0x78f:
-  // all but vector memory's) except where that is slower (8192 x 8192 by 32
-  // MX rows 9.4 us, from 8.9; by 64, tiles of 2 x 4, 12.0, and without 12.9).
-  constexpr int MAY_PASS = MODE == X_MX && MT == NT ? 0 : 0x78f;
+  // The next step's loads stay in front of a step's products (0x78f: all but
+  // vector memory's instructions may pass); left to itself the compiler puts
+  // them behind, which saves registers.
+  constexpr int MAY_PASS = 0x78f;
 
   S f[DEPTH];
 #pragma unroll
@@ -387,12 +385,12 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
 // and converts x once for all the weight rows of its tile, so that wide tiles
 // cost less a weight, but half as wide ones on twice the CUs take less time.
 // Up to a tile a CU its waves split K eight ways; with more, four ways, and
-// two tiles share a CU. K = 8192, us:
-//   64 MX rows: N = 5500 2x4 tiles 12.3, 2x2 15.0; 8192 2x4 12.3, 4x4 18.6;
-//     9000 4x4 18.3, 2x4 23.9; 18000 4x4 by four waves 31.5, by eight 34.3
-//   32: 4096 (K too) 1x2 4.5, 2x2 5.5; 8192 2x2 8.9, 2x4 12.0; 10000 2x4
-//     12.4, 2x2 14.8; 18000 bf16 2x4 by four waves 23.5, by eight 26.5
-//   16: 8192 1x2 8.1, 1x4 9.3; 10000 1x4 9.9, 1x2 11.7
+// two tiles share a CU. us, weights from memory, K = 8192 but where given:
+//   64 MX rows: N = 8192 2x4 tiles 15.0, 2x2 18.0; 12000 4x4 22.7, 2x4 25.8;
+//     28000 4x4 by four waves 43.8, by eight 44.6; 50000 (K = 4096) 42.9, 48.0
+//   32: 8192 2x2 12.3, 1x4 12.9; 12000 2x4 16.8, 2x2 21.0
+//   16: 8192 1x2 10.0, 1x4 13.3; 12000 1x4 14.5, 1x2 16.4
+//   64 bf16 rows: 28000 4x4 by four waves 52.8, by eight 56.1
 template <int MODE>
 hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
