@@ -931,3 +931,22 @@ def test_sample_greedy_takes_the_first_of_the_highest(dtype, v):
         x[7, 9:] = 0.0
     want = [(r == r.max()).nonzero()[0].item() for r in x.cpu().float()]
     assert ops.sample(x, _uniform(8, 89), temperature=0.0).tolist() == want
+
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+@pytest.mark.parametrize("m,n,k", [
+    (2, 4200, 1088), (5, 4099, 192), (9, 4200, 320), (16, 8300, 448), (20, 4200, 320),
+    (20, 8300, 2112), (32, 16501, 576), (33, 8300, 320), (40, 4200, 640), (64, 16333, 1088),
+    (64, 16500, 448), (61, 33001, 64), (130, 4200, 320)])
+def test_gemv_4bit_every_tile(m, n, k, act):
+    # widths at which each tile of the rule is taken, by four and eight waves
+    w4, sw = _weights(n, k, 90)
+    w64 = _fp4_values(w4, sw)
+    if act == "mx":
+        q, sq = _mx_acts(m, k, 91)
+        got, x64 = ops.gemv_mx_w4(q, sq, w4, sw), _mx_values(q, sq)
+    else:
+        x = _randn((m, k), 91, torch.bfloat16 if act == "bf16" else torch.float16)
+        got, x64 = ops.gemv_w4(x, w4, sw), x.double()
+    assert _product_ok(got, x64, w64)
