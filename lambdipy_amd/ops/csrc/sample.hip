@@ -17,7 +17,8 @@
 // occur. 256 x 131072 bf16: 33 us, 32 where 9 of 10 are masked, 14 greedy; of
 // the 26 in the kernel the LDS atomics of the counting take 11, reading the
 // row a second time for the index 5, the sums and exps of its 72 groups of 64
-// values 4. 1 x 32000: 15 us; 1 x 524288: 64 (115 as f32).
+// values 4 (with top-k fewer of them). 1 x 32000: 15 us, with top-k 14; 1 x
+// 524288: 64 (115 as f32).
 //
 // f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
 // bin that holds a border, and only that bin's members are looked at. An exp
@@ -132,7 +133,11 @@ __device__ __forceinline__ void scan(const T* __restrict__ row, int begin,
 #define LPX_ADD_32(ctrl, rows) v += LPX_FROM(v, ctrl, rows);
 #define LPX_MAX_32(ctrl, rows) v = max(v, LPX_FROM(v, ctrl, rows));
 
-// Running sums.
+// Running sums, of 16 lanes and of all.
+__device__ __forceinline__ unsigned row_run_up(unsigned v) {
+  LPX_ROW_STEPS(LPX_ADD_32)
+  return v;
+}
 __device__ __forceinline__ u64 wave_run_up(u64 v) {
   LPX_SIX_STEPS(LPX_ADD_64)
   return v;
@@ -869,7 +874,8 @@ __device__ __forceinline__ void find_border(TableShared& sh, const RowScale& r,
       // how many copies reach it: border - was of `each`, rounded up
       u64 need = border - was;
       if (!by_count) {
-        u64 q = (u64)((double)need / (double)w);
+        // an estimate (at most 2^19 copies), put right
+        u64 q = (u64)((float)need * __builtin_amdgcn_rcpf((float)w));
         while (q * w < need) ++q;
         while (q > 1 && (q - 1) * w >= need) --q;
         need = q;
@@ -1192,39 +1198,90 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
   const RowScale r = row_scale(a, row, e);
   const u64 least = least_weight(a, row, r);
   // Sums of groups of 64 ranks. A list of those that hold something, of which
-  // each wave takes its share: weights are most of the work.
+  // each wave takes its share: weights are most of the work. Where top-k cuts
+  // the row, the groups behind its border are left out, so members are counted
+  // first.
   constexpr int WAVES = ROW_THREADS / 64;
+  const double k = param(a.top_k, row);
+  const unsigned lowest_rank = sh.last, lowest_count = sh.lowest;
+  unsigned all = 0;
+  u64 minp = 0;
 #pragma unroll
   for (int i = 0; i < 128 / WAVES; ++i) {
     const int b = i * WAVES + wave;  // 16 lanes read 64 words
     const i32x4 c = *reinterpret_cast<const i32x4*>(sh.count + b * 256 + lane * 4);
-    const unsigned some = row_or((unsigned)(c[0] | c[1] | c[2] | c[3]));
-    if ((lane & 15) == 15 && some) {
-      const int group = b * 4 + lane / 16;
-      if (some & 0xffffu) sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)group;
-      if (some >> 16)
-        sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)(group + GROUPS / 2);
+    const int group = b * 4 + lane / 16;
+    if (r.by_k) {
+      const u16x2 ones = {1, 1}, upper = {0, 1};
+      unsigned both = 0, hi = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int word = c[j];
+        const u16x2 n = __builtin_bit_cast(u16x2, word);
+        both = __builtin_amdgcn_udot2(n, ones, both, false);
+        hi = __builtin_amdgcn_udot2(n, upper, hi, false);
+      }
+      all += both;
+      unsigned lo = both - hi;
+      // NaN and -inf are no members
+      const int first_word = b * 256 + lane * 4;
+      if (b * 256 < (int)Ranks<T>::INF) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (first_word + j < (int)Ranks<T>::INF) lo -= (unsigned)c[j] & 0xffffu;
+      }
+      if (b * 256 >= (int)(Ranks<T>::NONE & 0x7f00u)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (first_word + j >= (int)(Ranks<T>::NONE & 0x7fffu)) hi -= (unsigned)c[j] >> 16;
+      }
+      lo = row_run_up(lo);
+      hi = row_run_up(hi);
+      if ((lane & 15) == 15) {
+        sh.members[group] = lo;
+        sh.members[group + GROUPS / 2] = hi;
+      }
+    } else {
+      const unsigned some = row_or((unsigned)(c[0] | c[1] | c[2] | c[3]));
+      if ((lane & 15) == 15 && some) {
+        if (some & 0xffffu) sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)group;
+        if (some >> 16)
+          sh.group_list[atomicAdd(&sh.groups, 1u)] = (unsigned short)(group + GROUPS / 2);
+      }
     }
   }
   __syncthreads();
-  u64 minp = 0;
-  unsigned all = 0;
+  if (r.by_k) {
+    // in the table the lowest value is one
+    if (t == 0) all += lowest_count - 1u;
+    unsigned own = sh.members[t];
+    if (t == (int)(lowest_rank >> 6) && lowest_rank >= Ranks<T>::INF &&
+        lowest_rank < Ranks<T>::NONE)
+      own += lowest_count - 1u;
+    const unsigned through = block_run_up(own, sh.wave_members);
+    sh.members[t] = through;  // thread t has group t
+    const bool in = own && (double)(through - own) < k;
+    const u64 who = __ballot(in);
+    unsigned at = 0;
+    if (lane == 0 && who) at = atomicAdd(&sh.groups, (unsigned)__popcll(who));
+    at = __builtin_amdgcn_readfirstlane(at) +
+         __builtin_amdgcn_mbcnt_hi((unsigned)(who >> 32),
+                                   __builtin_amdgcn_mbcnt_lo((unsigned)who, 0u));
+    if (in) sh.group_list[at] = (unsigned short)t;
+    __syncthreads();
+  }
   const int groups = (int)sh.groups, share = (groups + WAVES - 1) / WAVES;
   for (int i = wave * share; i < min(groups, wave * share + share); ++i) {
     const int group = __builtin_amdgcn_readfirstlane(sh.group_list[i]);
     const unsigned rank = (unsigned)group * 64 + lane;
     unsigned n = count_at(sh, rank);
-    all += n;
+    if (!r.by_k) all += n;
     if (rank < Ranks<T>::INF || rank >= Ranks<T>::NONE) n = 0;
     const u64 w = weight(r, logit_at<T>(rank));
     u64 mass = n * w;
     if (w >= least) minp += mass;
     mass = wave_run_up(mass);
-    if (r.by_k) n = wave_run_up(n);
-    if (lane == 63) {
-      sh.mass[group] = mass;
-      sh.members[group] = n;
-    }
+    if (lane == 63) sh.mass[group] = mass;
   }
   all = wave_run_up(all);
   minp = wave_run_up(minp);
@@ -1238,17 +1295,10 @@ __global__ __launch_bounds__(ROW_THREADS) void row_table_kernel(SampleArgs a) {
     whole_row<T>(a, row, shared.row);
     return;
   }
-  // Running sums; thread t has group t
-  {
-    const u64 m = block_run_up(sh.mass[t], sh.wave_mass);
-    const unsigned n = r.by_k ? block_run_up(sh.members[t], sh.wave_members) : 0;
-    sh.mass[t] = m;
-    sh.members[t] = n;
-  }
+  sh.mass[t] = block_run_up(sh.mass[t], sh.wave_mass);  // as of members
   __syncthreads();
 
   u64 kept = sh.mass[GROUPS - 1];
-  const double k = param(a.top_k, row);
   if (r.by_k && k < (double)sh.members[GROUPS - 1]) {
     find_border<T>(sh, r, true, (u64)k);
     kept = sh.kept;
