@@ -14,9 +14,9 @@
 // neighbouring elements (16-B loads of 16-bit types), an MX block is four
 // neighbouring lanes, a 128-element scale tile sixteen. One step a thread and
 // as many threads as the row needs: 16384 x 8192 bf16 with residual to MX 204
-// us with 256 threads of four steps each, 174 with 1024 of one, 162 (5.8
-// TB/s) where the stores also pass by the caches; a copy of that size in
-// torch reaches 4.9.
+// us with 256 threads of four steps each, 174 with 1024 of one, 162 where
+// the stores also pass by the caches, 158 (6.0 TB/s) without the code for
+// widths that are no multiple of 8; a copy of that size in torch reaches 4.9.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -53,20 +53,26 @@ __device__ __forceinline__ void store8(T* p, f32x8 f) {
                               reinterpret_cast<words*>(p));
 }
 
-// Elements [c, c+8) of a row of K; what lies behind K is 0.
-template <typename T>
+// Elements [c, c+8) of a row of K; what lies behind K is 0. WHOLE: K is a
+// multiple of 8.
+template <bool WHOLE, typename T>
 __device__ __forceinline__ f32x8 load_row(const T* row, int c, int K) {
-  if (c + 8 <= K) return load8(row + c);
-  f32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (WHOLE || c + 8 <= K) return load8(row + c);
+  if ((K & 7) == 1) return f32x8{(float)row[c], 0, 0, 0, 0, 0, 0, 0};
+  // All are asked for before one is waited for, the last again in place of
+  // those behind it: 9999 x 5004 fp16 104 us with a branch each, 96 so.
+  T e[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < K) v[j] = (float)row[c + j];
+  for (int j = 0; j < 8; ++j) e[j] = row[min(c + j, K - 1)];
+  f32x8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = c + j < K ? (float)e[j] : 0.f;
   return v;
 }
 
-template <typename T>
+template <bool WHOLE, typename T>
 __device__ __forceinline__ void store_row(T* row, int c, int K, f32x8 v) {
-  if (c + 8 <= K) {
+  if (WHOLE || c + 8 <= K) {
     store8(row + c, v);
     return;
   }
@@ -145,27 +151,27 @@ struct NormArgs {
   bool weight_f32;
 };
 
-template <typename T, bool MX>
+template <typename T, bool MX, bool WHOLE>
 __device__ __forceinline__ void finish8(const NormArgs& a, int row, int c,
                                         f32x8 h, float inv) {
   f32x8 w = {0, 0, 0, 0, 0, 0, 0, 0};
   if (c < a.K)
-    w = a.weight_f32 ? load_row((const float*)a.weight, c, a.K)
-                     : load_row((const T*)a.weight, c, a.K);
+    w = a.weight_f32 ? load_row<WHOLE>((const float*)a.weight, c, a.K)
+                     : load_row<WHOLE>((const T*)a.weight, c, a.K);
   const f32x8 y = h * inv * w;
   if constexpr (MX)
     store_mx((unsigned char*)a.y + (long)row * a.K, a.sc, row, a.R, c, a.K, y);
   else if (c < a.K)
-    store_row((T*)a.y + (long)row * a.K, c, a.K, y);
+    store_row<WHOLE>((T*)a.y + (long)row * a.K, c, a.K, y);
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ f32x8 read_h(const NormArgs& a, int row, int c,
                                         bool keep) {
-  f32x8 h = load_row((const T*)a.x + (long)row * a.x_stride, c, a.K);
+  f32x8 h = load_row<WHOLE>((const T*)a.x + (long)row * a.x_stride, c, a.K);
   if (a.res) {
-    h += load_row((const T*)a.res + (long)row * a.res_stride, c, a.K);
-    if (keep) store_row((T*)a.h + (long)row * a.K, c, a.K, h);
+    h += load_row<WHOLE>((const T*)a.res + (long)row * a.res_stride, c, a.K);
+    if (keep) store_row<WHOLE>((T*)a.h + (long)row * a.K, c, a.K, h);
   }
   return h;
 }
@@ -178,21 +184,21 @@ __device__ __forceinline__ float square_sum(f32x8 h) {
 }
 
 // Rows of at most 512: `lanes` (a power of two, 8 at least) of a wave each.
-template <typename T, bool MX>
+template <typename T, bool MX, bool WHOLE>
 __global__ __launch_bounds__(256) void rmsnorm_short_kernel(NormArgs a, int lanes) {
   const int rows = 256 / lanes;
   const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x) * rows +
                   (int)threadIdx.x / lanes;
   const int c = row < a.R ? (int)threadIdx.x % lanes * 8 : a.K;
   f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
-  if (c < a.K) h = read_h<T>(a, row, c, true);
+  if (c < a.K) h = read_h<T, WHOLE>(a, row, c, true);
   float s = square_sum(h);
   for (int m = lanes / 2; m > 0; m >>= 1) s += __shfl_xor(s, m, 64);
-  finish8<T, MX>(a, row, c, h, rsqrtf(s / (float)a.K + a.eps));
+  finish8<T, MX, WHOLE>(a, row, c, h, rsqrtf(s / (float)a.K + a.eps));
 }
 
 // Rows of at most blockDim * STEPS * 8 elements.
-template <typename T, bool MX, int STEPS>
+template <typename T, bool MX, bool WHOLE, int STEPS>
 __global__ __launch_bounds__(1024) void rmsnorm_kernel(NormArgs a) {
   // neighbouring rows on one XCD: their scale bytes share lines of its L2
   const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
@@ -202,53 +208,60 @@ __global__ __launch_bounds__(1024) void rmsnorm_kernel(NormArgs a) {
   for (int i = 0; i < STEPS; ++i) {
     const int c = (int)(i * blockDim.x + threadIdx.x) * 8;
     h[i] = f32x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < a.K) h[i] = read_h<T>(a, row, c, true);
+    if (c < a.K) h[i] = read_h<T, WHOLE>(a, row, c, true);
     s += square_sum(h[i]);
   }
   const float inv = rsqrtf(block_sum(s) / (float)a.K + a.eps);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i)
-    finish8<T, MX>(a, row, (int)(i * blockDim.x + threadIdx.x) * 8, h[i], inv);
+    finish8<T, MX, WHOLE>(a, row, (int)(i * blockDim.x + threadIdx.x) * 8, h[i], inv);
 }
 
 // Longer rows: read a second time (the first pass left them in the caches).
-template <typename T, bool MX>
+template <typename T, bool MX, bool WHOLE>
 __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
   const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
   const int steps = (a.K + 8191) / 8192;
   float s = 0.f;
   for (int i = 0; i < steps; ++i) {
     const int c = (i * 1024 + (int)threadIdx.x) * 8;
-    if (c < a.K) s += square_sum(read_h<T>(a, row, c, true));
+    if (c < a.K) s += square_sum(read_h<T, WHOLE>(a, row, c, true));
   }
   const float inv = rsqrtf(block_sum(s) / (float)a.K + a.eps);
   for (int i = 0; i < steps; ++i) {
     const int c = (i * 1024 + (int)threadIdx.x) * 8;
     f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < a.K) h = read_h<T>(a, row, c, false);
-    finish8<T, MX>(a, row, c, h, inv);
+    if (c < a.K) h = read_h<T, WHOLE>(a, row, c, false);
+    finish8<T, MX, WHOLE>(a, row, c, h, inv);
   }
 }
 
-template <typename T, bool MX>
+template <typename T, bool MX, bool WHOLE>
 hipError_t launch(const NormArgs& a, hipStream_t stream) {
   const int threads = (a.K + 7) / 8;
   if (threads <= 64) {
     int lanes = 8;
     while (lanes < threads) lanes *= 2;
     const int rows = 256 / lanes;
-    rmsnorm_short_kernel<T, MX>
+    rmsnorm_short_kernel<T, MX, WHOLE>
         <<<dim3((unsigned)((a.R + rows - 1) / rows)), dim3(256), 0, stream>>>(a, lanes);
     return hipGetLastError();
   }
   const dim3 grid((unsigned)a.R), block((unsigned)((threads + 63) / 64 * 64)), most(1024);
   if (threads <= 1024)
-    rmsnorm_kernel<T, MX, 1><<<grid, block, 0, stream>>>(a);
+    rmsnorm_kernel<T, MX, WHOLE, 1><<<grid, block, 0, stream>>>(a);
   else if (threads <= 2048)
-    rmsnorm_kernel<T, MX, 2><<<grid, most, 0, stream>>>(a);
+    rmsnorm_kernel<T, MX, WHOLE, 2><<<grid, most, 0, stream>>>(a);
   else
-    rmsnorm_long_kernel<T, MX><<<grid, most, 0, stream>>>(a);
+    rmsnorm_long_kernel<T, MX, WHOLE><<<grid, most, 0, stream>>>(a);
   return hipGetLastError();
+}
+
+template <typename T, bool MX>
+hipError_t by_width(const NormArgs& a, hipStream_t stream) {
+  if constexpr (!MX)  // whose rows are whole blocks
+    if (a.K % 8 != 0) return launch<T, MX, false>(a, stream);
+  return launch<T, MX, true>(a, stream);
 }
 
 template <bool MX>
@@ -256,9 +269,9 @@ hipError_t by_type(ActType t, const NormArgs& a, hipStream_t stream) {
   if (a.R <= 0) return hipSuccess;
   if (a.K <= 0 || (MX && a.K % 64 != 0)) return hipErrorInvalidValue;
   switch (t) {
-    case ActType::bf16: return launch<__bf16, MX>(a, stream);
-    case ActType::f16: return launch<_Float16, MX>(a, stream);
-    case ActType::f32: return launch<float, MX>(a, stream);
+    case ActType::bf16: return by_width<__bf16, MX>(a, stream);
+    case ActType::f16: return by_width<_Float16, MX>(a, stream);
+    case ActType::f32: return by_width<float, MX>(a, stream);
   }
   return hipErrorInvalidValue;
 }
