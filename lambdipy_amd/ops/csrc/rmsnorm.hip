@@ -12,11 +12,12 @@
 // The row stays in registers between the two uses of it, so each input is
 // read once and each output written once; memory bounds it. A thread owns 8
 // neighbouring elements (16-B loads of 16-bit types), an MX block is four
-// neighbouring lanes, a 128-element scale tile sixteen. One step a thread and
-// as many threads as the row needs: 16384 x 8192 bf16 with residual to MX 204
-// us with 256 threads of four steps each, 174 with 1024 of one, 162 where
-// the stores also pass by the caches, 158 (6.0 TB/s) without the code for
-// widths that are no multiple of 8; a copy of that size in torch reaches 4.9.
+// neighbouring lanes, a 128-element scale tile sixteen. A thread takes one
+// step, or two, and a row as many threads as it needs: 16384 x 8192 bf16 with
+// residual to MX 204 us with 256 threads of four steps each, 174 with 1024 of
+// one, 162 where the stores also pass by the caches, 158 (6.0 TB/s) without
+// the code for widths that are no multiple of 8; a copy of that size in torch
+// reaches 4.9.
 
 #include "lpx_common.h"
 #include "kernels.h"
@@ -236,6 +237,21 @@ __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
   }
 }
 
+// Whether rows of up to 1024 threads of one step are better done by half as
+// many of two. Rows that the chip holds at once are not (512 x 5120 bf16 5.6
+// us, 6.7 by two). Where that leaves a second round with little in it they
+// are: 1030 x 4096 bf16 6.2 and 5.1, 2048 x 4096 14.2 and 16.1, 1000 x 7168
+// 13.7 and 11.5, 8192 x 7168 84 and 88. So they are, however many, at 10 to 12
+// waves, of which a CU takes two workgroups only (8192 x 5120 to MX 64 and 58;
+// f32 63 and 67), and at widths off the loads' 8 (9999 x 5003 fp16 106 and 91).
+template <typename T, bool WHOLE>
+bool two_steps(int R, int waves) {
+  const int slots = 256 * (waves > 9 ? 2 : 32 / waves);
+  if (R <= slots) return false;
+  if (sizeof(T) == 2 && (!WHOLE || (waves >= 10 && waves <= 12))) return true;
+  return R <= (waves > 8 ? 2 * slots : slots + slots / 4);
+}
+
 template <typename T, bool MX, bool WHOLE>
 hipError_t launch(const NormArgs& a, hipStream_t stream) {
   const int threads = (a.K + 7) / 8;
@@ -247,8 +263,12 @@ hipError_t launch(const NormArgs& a, hipStream_t stream) {
         <<<dim3((unsigned)((a.R + rows - 1) / rows)), dim3(256), 0, stream>>>(a, lanes);
     return hipGetLastError();
   }
-  const dim3 grid((unsigned)a.R), block((unsigned)((threads + 63) / 64 * 64)), most(1024);
-  if (threads <= 1024)
+  const int waves = (threads + 63) / 64;
+  const dim3 grid((unsigned)a.R), block((unsigned)waves * 64), most(1024);
+  if (threads <= 1024 && two_steps<T, WHOLE>(a.R, waves))
+    rmsnorm_kernel<T, MX, WHOLE, 2>
+        <<<grid, dim3((unsigned)(waves + 1) / 2 * 64), 0, stream>>>(a);
+  else if (threads <= 1024)
     rmsnorm_kernel<T, MX, WHOLE, 1><<<grid, block, 0, stream>>>(a);
   else if (threads <= 2048)
     rmsnorm_kernel<T, MX, WHOLE, 2><<<grid, most, 0, stream>>>(a);

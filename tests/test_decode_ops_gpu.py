@@ -950,3 +950,22 @@ def test_gemv_4bit_every_tile(m, n, k, act):
         x = _randn((m, k), 91, torch.bfloat16 if act == "bf16" else torch.float16)
         got, x64 = ops.gemv_w4(x, w4, sw), x.double()
     assert _product_ok(got, x64, w64)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,k", [(777, 5003), (1030, 4096), (600, 5120), (600, 7171),
+                                    (4200, 1003), (2600, 5122), (513, 8192), (9, 5004)])
+def test_rmsnorm_more_rows_than_fit_at_once(rows, k, dtype, residual):
+    # two steps a thread, and ragged ends of every length
+    test_rmsnorm(rows, k, dtype, residual)
+    test_rmsnorm(5, k + 1, dtype, residual)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("rows,k", [(1030, 4096), (600, 5120), (600, 7232), (4200, 1024)])
+def test_rmsnorm_mx_more_rows_than_fit_at_once(rows, k, dtype, residual):
+    test_rmsnorm_mx(rows, k, dtype, residual)
