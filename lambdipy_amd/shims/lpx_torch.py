@@ -267,10 +267,12 @@ class LinearW4:
     """Serving Linear on the mixed MX GEMM: weights quantized ONCE to
     fp4-MX (half the resident bytes and half the weight traffic of fp8),
     activations quantized per call to fp8-MX by the 9-TB/s hw quantizer.
-    Runs at the full fp8 MFMA rate (gemm_mx_w4: 1944/2293 TF @4096/8192).
+    Runs at the full fp8 MFMA rate (gemm_mx_w4: 1944/2293 TF @4096/8192) for
+    batches of whole tiles (batch % 256 == 0, the 8-phase scaled-MFMA tile).
+    Other batches, single tokens among them, read the same weights through
+    gemv_mx_w4 (8192 x 8192 by 16 rows: 8.3 us).
 
-    Requires serving-aligned shapes: batch % 256 == 0, out_features % 256
-    == 0, in_features % 128 == 0 (the 8-phase scaled-MFMA tile).
+    Requires out_features % 256 == 0, in_features % 128 == 0.
     """
 
     def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
@@ -284,10 +286,13 @@ class LinearW4:
         self.bias = bias
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        # x: [M, in_features] f32, M % 256 == 0
+        # x: [M, in_features] f32
         e = _ops.ext()
         qa, sa = e.quantize_mx(x.contiguous())
-        y = e.gemm_mx_w4(qa, sa, self.wq4, self.wsc4)
+        if x.shape[0] % 256 == 0:
+            y = e.gemm_mx_w4(qa, sa, self.wq4, self.wsc4)
+        else:
+            y = e.gemv_mx_w4(qa, sa, self.wq4, self.wsc4)
         if self.bias is not None:
             y = y + self.bias
         return y

@@ -969,3 +969,23 @@ def test_rmsnorm_more_rows_than_fit_at_once(rows, k, dtype, residual):
 @pytest.mark.parametrize("rows,k", [(1030, 4096), (600, 5120), (600, 7232), (4200, 1024)])
 def test_rmsnorm_mx_more_rows_than_fit_at_once(rows, k, dtype, residual):
     test_rmsnorm_mx(rows, k, dtype, residual)
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 7, 64, 200, 256])
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear_w4_of_any_batch(m, bias):
+    from lambdipy_amd.shims.lpx_torch import LinearW4
+
+    w, b = _randn((512, 384), 95, scale=0.05), _randn((512,), 96) if bias else None
+    lin, x = LinearW4(w, b), _randn((m, 384), 97)
+    got = lin(x)
+    qa, sa = ops.quantize_mx(x)
+    if m % 256:  # whole tiles go through the scaled MFMA, which sums less exactly
+        assert _product_ok(got if b is None else lin.__class__(w)(x), _mx_values(qa, sa),
+                           _fp4_values(lin.wq4, lin.wsc4))
+        y = ops.gemv_mx_w4(qa, sa, lin.wq4, lin.wsc4)
+    else:
+        y = ops.gemm_mx_w4(qa, sa, lin.wq4, lin.wsc4)
+    assert got.dtype == torch.float32
+    assert torch.equal(got, y if b is None else y + b)
