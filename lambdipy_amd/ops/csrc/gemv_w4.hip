@@ -385,12 +385,14 @@ hipError_t launch(const W4Args& a, hipStream_t stream) {
 // and converts x once for all the weight rows of its tile, so that wide tiles
 // cost less a weight, but half as wide ones on twice the CUs take less time.
 // Up to a tile a CU its waves split K eight ways; with more, four ways, and
-// two tiles share a CU. us, weights from memory, K = 8192 but where given:
+// two tiles share a CU; where half of the CUs have none, sixteen ways. us, weights from memory, K = 8192 but where given:
 //   64 MX rows: N = 8192 2x4 tiles 15.0, 2x2 18.0; 12000 4x4 22.7, 2x4 25.8;
 //     28000 4x4 by four waves 43.8, by eight 44.6; 50000 (K = 4096) 42.9, 48.0
 //   32: 8192 2x2 12.3, 1x4 12.9; 12000 2x4 16.8, 2x2 21.0
 //   16: 8192 1x2 10.0, 1x4 13.3; 12000 1x4 14.5, 1x2 16.4
+//     2000 1x1 by sixteen waves 6.0, by eight 6.4
 //   64 bf16 rows: 28000 4x4 by four waves 52.8, by eight 56.1
+//   1: 1000 by sixteen waves 4.3, by eight 4.5; fp16 4.8, 5.3
 template <int MODE>
 hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M <= 0 || a.N <= 0) return hipSuccess;
@@ -403,8 +405,9 @@ hipError_t by_size(const W4Args& a, hipStream_t stream) {
   // Rows that one load of x holds: 100000 x 8192 by one bf16 row 73 us,
   // loading a tile of 16 rows of x 80 us.
   if (a.M <= (MODE == X_MX ? 8 : 4))
-    return fills(1, 2) ? launch<MODE, 1, 2, 8, 2, true>(a, stream)
-                       : launch<MODE, 1, 1, 8, 2, true>(a, stream);
+    return fills(1, 2)   ? launch<MODE, 1, 2, 8, 2, true>(a, stream)
+           : fills(1, 1) ? launch<MODE, 1, 1, 8, 2, true>(a, stream)
+                         : launch<MODE, 1, 1, 16, 2, true>(a, stream);
   if constexpr (MODE != X_F16)  // whose scaled sums do not fit the registers
     if (a.M > 32 && fills(4, 4))
       return tiles(4, 4) > CUS ? launch<MODE, 4, 4, 4, 1>(a, stream)
@@ -417,7 +420,8 @@ hipError_t by_size(const W4Args& a, hipStream_t stream) {
   if (a.M > 16 && fills(2, 2)) return launch<MODE, 2, 2, 8, 1>(a, stream);
   if (fills(1, 4)) return launch<MODE, 1, 4, 8, 1>(a, stream);
   if (fills(1, 2)) return launch<MODE, 1, 2, 8, 1>(a, stream);
-  return launch<MODE, 1, 1, 8, 1>(a, stream);
+  if (fills(1, 1)) return launch<MODE, 1, 1, 8, 1>(a, stream);
+  return launch<MODE, 1, 1, 16, 2>(a, stream);
 }
 
 }  // namespace

@@ -989,3 +989,12 @@ def test_linear_w4_of_any_batch(m, bias):
         y = ops.gemm_mx_w4(qa, sa, lin.wq4, lin.wsc4)
     assert got.dtype == torch.float32
     assert torch.equal(got, y if b is None else y + b)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 8192), (1, 15, 2112), (3, 600, 64), (16, 2000, 4160),
+                                   (9, 600, 8192), (30, 500, 6144), (64, 65, 1088)])
+def test_gemv_4bit_few_tiles(m, n, k, act):
+    # sixteen ways along k
+    test_gemv_4bit_every_tile(m, n, k, act)
