@@ -57,6 +57,16 @@ struct ChunkBins {
   u64 minp;  // mass of w >= min_p
 };
 
+struct RowScale {
+  float hi;       // the row's largest logit
+  float per_bin;  // bins per unit of x
+  double hi64;    // a number over f32's where that is infinite
+  double per_x;   // powers of two per unit of x
+  double shift;
+  int at;
+  bool greedy, by_k, by_p;
+};
+
 struct SampleArgs {
   const void* logits;
   long stride;  // elements
@@ -64,6 +74,8 @@ struct SampleArgs {
   SampleParam temperature, top_k, top_p, min_p, u;
   ChunkMax* maxima;  // [rows][chunks]
   ChunkBins* bins;   // [rows][chunks]
+  RowScale* scales;  // [rows]
+  bool binned;       // the last two are there
   int64_t* token;
 };
 
@@ -181,16 +193,6 @@ struct Extent {
     for (int m = 32; m > 0; m >>= 1)
       join(__shfl_xor(hi, m, 64), __shfl_xor(lo, m, 64), __shfl_xor(at, m, 64));
   }
-};
-
-struct RowScale {
-  float hi;       // the row's largest logit
-  float per_bin;  // bins per unit of x
-  double hi64;    // a number over f32's where that is infinite
-  double per_x;   // powers of two per unit of x
-  double shift;
-  int at;
-  bool greedy, by_k, by_p;
 };
 
 constexpr double INFINITE = 1e300;
@@ -346,6 +348,7 @@ __global__ __launch_bounds__(CHUNK_THREADS) void chunk_bins_kernel(SampleArgs a)
   const ChunkMax* maxima = a.maxima + (long)row * a.chunks;
   const ChunkMax own = maxima[min((int)threadIdx.x & 63, a.chunks - 1)];
   const RowScale r = row_scale(a, row, row_extent(a, row, own));
+  if (begin == 0 && threadIdx.x == 0) a.scales[row] = r;
   if (r.greedy) return;
   __shared__ ChunkBins b;
   b.mass[threadIdx.x] = 0;
@@ -701,8 +704,13 @@ template <typename T>
 __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
   __shared__ RowShared sh;
   const int row = (int)blockIdx.x, t = (int)threadIdx.x;
-  const ChunkMax* maxima = a.maxima + (long)row * a.chunks;
-  const ChunkMax own = maxima[min(t & 63, a.chunks - 1)];
+  if (!a.binned) {  // greedy, as the host knows
+    const ChunkMax* maxima = a.maxima + (long)row * a.chunks;
+    const Extent e = row_extent(a, row, maxima[min(t & 63, a.chunks - 1)]);
+    if (t == 0) a.token[row] = row_scale(a, row, e).at;
+    return;
+  }
+  const RowScale r = a.scales[row];
   // thread t sums bin t % BINS over a quarter of the chunks
   const ChunkBins* c = a.bins + (long)row * a.chunks;
   const int bin = t % BINS;
@@ -727,7 +735,6 @@ __global__ __launch_bounds__(ROW_THREADS) void row_pick_kernel(SampleArgs a) {
     }
   }
   clear(sh.row);
-  const RowScale r = row_scale(a, row, row_extent(a, row, own));
   if (r.greedy) {
     if (t == 0) a.token[row] = r.at;
     return;
@@ -1359,9 +1366,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   } else {
     const dim3 grid((unsigned)a.chunks * (unsigned)a.rows);
     chunk_max_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
-    const SampleParam& t = a.temperature;
-    if (t.kind != SampleParam::value_ || t.value > 0)  // not known to be greedy
-      chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
+    if (a.binned) chunk_bins_kernel<T><<<grid, dim3(CHUNK_THREADS), 0, stream>>>(a);
     row_pick_kernel<T><<<rows, threads, 0, stream>>>(a);
   }
   return hipGetLastError();
@@ -1369,7 +1374,7 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
 
 struct Plan {
   int chunk, chunks;
-  size_t maxima_bytes, bytes;
+  size_t bins_at, scales_at, bytes;
 };
 
 Plan plan_of(ActType t, int rows, int vocab) {
@@ -1380,8 +1385,9 @@ Plan plan_of(ActType t, int rows, int vocab) {
   const long want = ((long)rows * vocab + 2047) / 2048;
   p.chunk = want <= 4096 ? 4096 : (int)(((want < vocab ? want : vocab) + 511) / 512 * 512);
   p.chunks = (vocab + p.chunk - 1) / p.chunk;
-  p.maxima_bytes = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
-  p.bytes = p.maxima_bytes + (size_t)rows * p.chunks * sizeof(ChunkBins);
+  p.bins_at = ((size_t)rows * p.chunks * sizeof(ChunkMax) + 255) / 256 * 256;
+  p.scales_at = p.bins_at + (size_t)rows * p.chunks * sizeof(ChunkBins);
+  p.bytes = p.scales_at + (size_t)rows * sizeof(RowScale);
   return p;
 }
 
@@ -1402,11 +1408,13 @@ hipError_t sample(ActType t, const void* logits, long stride, int rows,
   if ((int64_t)rows * p.chunks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
   int shift = 45;  // sums of `vocab` weights stay below 2^62
   while (vocab > (int64_t(1) << (62 - shift))) --shift;
+  char* const work = static_cast<char*>(workspace);
   SampleArgs a{logits, stride, rows, vocab, p.chunk, p.chunks, shift,
                temperature, top_k, top_p, min_p, u,
-               static_cast<ChunkMax*>(workspace),
-               reinterpret_cast<ChunkBins*>(static_cast<char*>(workspace) +
-                                            p.maxima_bytes),
+               reinterpret_cast<ChunkMax*>(work),
+               reinterpret_cast<ChunkBins*>(work + p.bins_at),
+               reinterpret_cast<RowScale*>(work + p.scales_at),
+               temperature.kind != SampleParam::value_ || temperature.value > 0,
                token};
   switch (t) {
     case ActType::bf16: return launch<__bf16>(a, stream);
