@@ -303,20 +303,24 @@ def fetch(name, output, version, py_tag, arch, release_dir):
               help="output path (single input only; default: in place)")
 @click.option("--json", "as_json", is_flag=True)
 def strip_archs(paths, archs, output, as_json):
-    """Strip non-target GPU code from HIP shared libraries.
+    """Strip non-target GPU code from HIP libraries that you built.
 
-    ROCm DSOs carry clang-offload fat binaries for ~14 gfx architectures;
-    for MI355X-only layers everything but gfx950 is dead weight (e.g.
-    libtorch_hip.so: 251 MB of fatbin -> ~26 MB). Rewrites the ELF in
-    place: rebundles each fat-binary entry, repoints the registration
-    wrappers/relocs, and compacts the file."""
-    from .packager.fatbin import strip_fatbin
+    A library compiled for several gfx architectures carries a code object
+    for each; for MI355X-only layers everything but gfx950 is dead weight.
+    Rewrites the ELF in place: rebundles each fat-binary entry, repoints the
+    registration wrappers/relocs, and compacts the file. The library's source
+    (NAME.hip, .cu, .cc or .cpp for libNAME.so) has to stand next to it:
+    compiled code of another origin is refused."""
+    from .packager.fatbin import ForeignLibrary, strip_fatbin
 
     if output and len(paths) != 1:
         raise click.ClickException("-o requires exactly one input")
     rows = []
     for p in paths:
-        st = strip_fatbin(p, output if output else None, archs=tuple(archs))
+        try:
+            st = strip_fatbin(p, output if output else None, archs=tuple(archs))
+        except ForeignLibrary as e:
+            raise click.ClickException(str(e))
         rows.append(st)
         if not as_json:
             click.echo(f"{p}: {st['old_size']/1e6:.1f} -> {st['new_size']/1e6:.1f} MB "

@@ -1,21 +1,23 @@
-"""gfx950-only fat-binary stripping for HIP shared libraries.
+"""gfx950-only fat binaries for HIP shared libraries that were built here.
 
-ROCm ships every GPU library with clang-offload-bundle fat binaries for
-~14 gfx architectures (libtorch_hip.so alone carries a 251 MB ``.hip_fatbin``
-section; the full torch dist is 11.5 GB).  For an MI355X-only deployment
-everything except the ``gfx950`` entries is dead weight.  This module
-rewrites a DSO in place of that weight (reference parity: lambdipy trims
-library payloads to fit Lambda's 250 MB layer limit — see SURVEY.md §2.2 N6
-"strip/prune pass"; this is the MI355X-native equivalent for HIP fat
-binaries, which the reference never had to deal with).
+hipcc puts one code object per ``--offload-arch`` into a library's
+``.hip_fatbin`` section. For an MI355X-only deployment everything but the
+``gfx950`` entries is dead weight, and a layer has a size limit (reference
+parity: lambdipy trims library payloads to fit Lambda's 250 MB layer limit).
 
-Mechanics (empirically verified against ROCm 7.2 libtorch_hip.so):
+Only a library whose source is at hand is rewritten: ``lib<name>.so`` (or
+``<name>.so``) next to ``<name>.hip``, ``.cu``, ``.cc`` or ``.cpp``, no older
+than that. Compiled code of another origin, an installed library or one out of
+a wheel, is not taken apart: strip_fatbin refuses it before it reads more than
+the names of its sections.
+
+Mechanics:
   - ``.hipFatBinSegment`` holds 24-byte wrappers {magic 0x48495046, version,
     ptr, reserved}; ``ptr`` is the vaddr of a bundle inside ``.hip_fatbin``,
     applied at load time through a R_X86_64_RELATIVE reloc whose addend
-    equals that vaddr.
-  - bundles are zstd-"CCOB" compressed offload bundles (or raw
-    ``__CLANG_OFFLOAD_BUNDLE__`` archives); each carries one entry per arch
+    equals that vaddr, or a R_X86_64_64 one against a symbol with that value.
+  - bundles are compressed offload bundles ("CCOB") or raw
+    ``__CLANG_OFFLOAD_BUNDLE__`` archives; each carries one entry per arch
     plus an empty host stub.
   - we unbundle/rebundle each through ``clang-offload-bundler`` keeping only
     the host stub + requested archs, rewrite the section, repoint wrappers
@@ -27,12 +29,9 @@ Mechanics (empirically verified against ROCm 7.2 libtorch_hip.so):
 
 The result dlopens and runs kernels exactly as before on gfx950 machines.
 
-When the DSO has no PT_NOTE to reuse (e.g. libmagma.so), the section is
-rewritten in place and its tail zero-filled: the file size is unchanged but
-the zeros cost nothing after zip/zstd in the layer artifact. Measured on
-the ROCm 7.2 torch dist (torch/lib): 5.43 -> 3.73 GB on disk
-(libtorch_hip 423->200 MB, rocsolver 760->90, rocsparse 392->80,
-rocrand 354->42, MIOpen 954->797, rocblas 55->30; magma zero-filled).
+When the library has no PT_NOTE to reuse, the section is rewritten in place
+and its tail zero-filled: the file size is unchanged but the zeros cost
+nothing after zip/zstd in the layer artifact.
 """
 
 from __future__ import annotations
@@ -53,6 +52,34 @@ PAGE = 4096
 PT_LOAD, PT_NOTE = 1, 4
 R_X86_64_64 = 1
 R_X86_64_RELATIVE = 8
+SOURCES = (".hip", ".cu", ".cc", ".cpp")
+
+
+class ForeignLibrary(ValueError):
+    """A library with GPU code that was not built here from its source."""
+
+
+def source_of(path: str) -> Optional[str]:
+    """The source next to a library from which it was built, or None."""
+    real = os.path.realpath(path)
+    folder, name = os.path.split(real)
+    stem = name.split(".so")[0]
+    stems = {stem, stem[3:]} if stem.startswith("lib") else {stem}
+    for s in sorted(stems):
+        for ext in SOURCES:
+            src = os.path.join(folder, s + ext)
+            if s and os.path.isfile(src) and (
+                os.path.getmtime(src) <= os.path.getmtime(real)
+            ):
+                return src
+    return None
+
+
+def has_fat_binary(path: str) -> bool:
+    """Whether a library has HIP code in it, by the names of its sections."""
+    out = subprocess.run(["readelf", "-S", "-W", path], capture_output=True,
+                         text=True, check=True).stdout
+    return ".hip_fatbin" in out.split()
 
 
 @dataclass
@@ -202,8 +229,18 @@ def strip_fatbin(src: str, dst: Optional[str] = None,
     """Strip non-`archs` GPU code from a HIP DSO. Returns a stats dict.
 
     Writes to `dst` (default: in-place via temp + rename). No-op (still
-    copies) when the DSO has no .hip_fatbin section.
+    copies) when the DSO has no .hip_fatbin section. Raises ForeignLibrary
+    when it has one but no source next to it.
     """
+    if not has_fat_binary(src):
+        if dst and dst != src:
+            shutil.copyfile(src, dst)
+        size = os.path.getsize(src)
+        return {"src": src, "old_size": size, "new_size": size, "bundles": 0,
+                "stripped": 0}
+    if source_of(src) is None:
+        raise ForeignLibrary(
+            f"{src}: no source next to it; only libraries built here are stripped")
     with open(src, "rb") as f:
         data = bytearray(f.read())
     e = _parse_elf(data)
@@ -218,8 +255,8 @@ def strip_fatbin(src: str, dst: Optional[str] = None,
 
     # 1. wrappers -> bundle vaddrs. The in-file ptr field may be zero (set
     # only at load time), so resolve via the reloc targeting it: either a
-    # RELATIVE addend (libtorch_hip style) or an R_X86_64_64 against a
-    # dynsym whose st_value is the bundle vaddr (librccl style).
+    # RELATIVE addend or an R_X86_64_64 against a dynsym whose st_value is
+    # the bundle vaddr.
     rela = e.section(".rela.dyn")
     dynsym = e.section(".dynsym")
     rel_by_off: Dict[int, int] = {}

@@ -6,8 +6,7 @@ MIOpen/rocsolver/rocsparse add another ~1.7 GB. The dynamic loader only
 needs the DEFINED SYMBOLS to resolve, so a deployment layer can ship a
 kilobyte-sized stub that exports the same symbol set (functions trap if
 ever called; data symbols are zeroed storage of the original size) under
-the same SONAME. Combined with fatbin.strip_fatbin this shrinks a working
-gfx950 torch runtime from 11.5 GB to roughly a gigabyte.
+the same SONAME.
 
 Reference parity: lambdipy prunes wheel payloads to fit Lambda limits
 (SURVEY.md §2.2 N6); stubbing is the MI355X-native extension of that idea

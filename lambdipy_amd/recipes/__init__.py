@@ -35,6 +35,10 @@ from packaging.specifiers import SpecifierSet
 from packaging.utils import canonicalize_name
 from packaging.version import InvalidVersion, Version
 
+from ..utils.log import get_logger
+
+log = get_logger("recipes")
+
 RECIPE_FORMAT = 1
 DATA_DIR = os.path.join(os.path.dirname(__file__), "data")
 
@@ -60,7 +64,6 @@ class BuildRecipe:
     excludes: List[str] = field(default_factory=list)
     prune: List[str] = field(default_factory=list)
     strip_native: bool = True
-    strip_archs: bool = False  # strip non-gfx950 HIP fat-binary entries
     stub_native: List[str] = field(default_factory=list)  # deps to stub out
     vendor_upstream: bool = True  # False: upstream pkg is runtime-provided
     runtime_requires: List[str] = field(default_factory=list)
@@ -80,6 +83,9 @@ class BuildRecipe:
         if d["kind"] not in _ALLOWED_KINDS:
             raise RecipeError(f"recipe {d['name']}: kind must be one of {sorted(_ALLOWED_KINDS)}")
         SpecifierSet(d["versions"])  # validate
+        if d.get("strip_archs"):
+            log.warning("recipe %s: strip_archs has no effect (libraries out of "
+                        "wheels are not rewritten)", d["name"])
         r = cls(
             name=canonicalize_name(d["name"]),
             versions=d["versions"],
@@ -90,7 +96,6 @@ class BuildRecipe:
             excludes=[canonicalize_name(e) for e in d.get("excludes", [])],
             prune=list(d.get("prune", [])),
             strip_native=bool(d.get("strip_native", True)),
-            strip_archs=bool(d.get("strip_archs", False)),
             stub_native=list(d.get("stub_native", [])),
             vendor_upstream=bool(d.get("vendor_upstream", True)),
             runtime_requires=list(d.get("runtime_requires", [])),
