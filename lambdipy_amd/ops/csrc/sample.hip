@@ -208,7 +208,8 @@ __device__ __forceinline__ RowScale row_scale(const SampleArgs& a, int row,
   r.greedy = !(t > 0) || r.at < 0;
   r.by_k = param(a.top_k, row) >= 1;
   r.by_p = param(a.top_p, row) < 1;
-  r.per_x = fmin(1.4426950408889634 / t, 1e300);  // 1 / (T ln 2)
+  // 1 / (T ln 2); beside +inf a finite logit weighs nothing at any T
+  r.per_x = e.hi == __builtin_inff() ? 1.0 : fmin(1.4426950408889634 / t, 1e300);
   r.shift = a.shift;
   // Below 32 T the weight rounds to nothing (e^-32 < 2^-46). A range that is
   // nothing or infinite is one bin.
@@ -252,8 +253,11 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {
 // another.
 __device__ __forceinline__ u64 weight(const RowScale& r, float x) {
 #pragma clang fp contract(off)
-  const double d = fmin((double)x, INFINITE) - r.hi64;
-  // 2^-2 and less rounds to nothing; fmax takes the number of the two
+  // NaN becomes -inf here: left to the arithmetic it is +inf, as fmin takes
+  // the number of the two
+  const double d = fmin((double)(real(x) ? x : -__builtin_inff()), INFINITE) - r.hi64;
+  // 2^-2 and less rounds to nothing; so does -inf at an infinite T, where the
+  // product is NaN
   const double y = fmax(__builtin_fma(d, r.per_x, r.shift), -2.0);
   const double n = __builtin_rint(y), f = y - n;
   // (2^f - 1) / f on [-1/2, 1/2], the polynomial of degree 8 through nine

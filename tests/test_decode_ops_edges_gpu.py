@@ -1,0 +1,91 @@
+"""The decode-step operators at the ends of what they take."""
+
+import pytest
+import torch
+
+from lambdipy_amd import ops
+from tests.test_decode_ops_gpu import DEV, _randn, gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+# ---- sampling: NaN beside infinities ----------------------------------------
+
+# how a row is sampled: f32 in one workgroup or as chunks; 16 bits by the count
+# of each value, or as f32 because one value is there more than 65535 times
+SAMPLE_FORMS = [("whole", torch.float32, 3001), ("chunks", torch.float32, 50001),
+                ("many chunks", torch.float32, 400003),
+                ("bf16", torch.bfloat16, 30001), ("fp16", torch.float16, 30001),
+                ("bf16 kept whole", torch.bfloat16, 140001),
+                ("fp16 kept whole", torch.float16, 140001)]
+
+
+def _finite_row(dtype, v, seed):
+    x = _randn((v,), seed, dtype)
+    if dtype != torch.float32 and v > 65536:
+        x[torch.arange(70000) * 2] = 1.0
+        x[1::2] = x[1::2].clamp(-4, -0.5)
+    return x
+
+
+def _mids(n):
+    """One u in the middle of each of n equal shares."""
+    return ((torch.arange(n) + 0.5) / n).to(DEV)
+
+
+def _every_third(v, n, start):
+    return [start + i * (v // (3 * n)) for i in range(n)]
+
+
+@gpu
+@pytest.mark.parametrize("form,dtype,v", SAMPLE_FORMS)
+@pytest.mark.parametrize("infs,nans", [(2, 1), (3, 40), (100, 300)])
+def test_sample_infinities_share_a_row_beside_nan(form, dtype, v, infs, nans):
+    row = _finite_row(dtype, v, 300)
+    at_inf, at_nan = _every_third(v, infs, 7), _every_third(v, nans, v // 2)
+    row[at_nan] = NAN
+    row[at_inf] = INF
+    for settings, n in ((dict(), infs), (dict(temperature=0.1), infs),
+                        (dict(top_k=2), 2), (dict(top_k=infs + 1), infs),
+                        (dict(top_k=infs + nans + 5), infs),
+                        (dict(top_p=(infs - 0.5) / infs), infs),
+                        (dict(top_p=1.5 / infs), 2), (dict(min_p=0.5), infs),
+                        (dict(top_k=infs + nans, top_p=0.999, min_p=0.1), infs)):
+        u = _mids(n)
+        got = ops.sample(row.expand(n, v), u, **settings)
+        assert got.tolist() == at_inf[:n], settings
+
+
+@gpu
+@pytest.mark.parametrize("form,dtype,v", SAMPLE_FORMS)
+def test_sample_at_endless_temperatures(form, dtype, v):
+    # all that a token can be drawn from is alike; with +inf that alone
+    row = _finite_row(dtype, v, 301)
+    row[_every_third(v, 50, 11)] = NAN
+    row[_every_third(v, 30, v // 2)] = -INF
+    order = torch.sort(torch.where(row.isnan(), -INF, row.float()).cpu(), descending=True,
+                       stable=True).indices
+    n = v - 80
+    u = torch.tensor([0.25 / n, 0.3, 0.77, 1 - 0.25 / n], dtype=torch.float64, device=DEV)
+    want = order[(u.cpu() * n).long()].tolist()
+    top = row.clone()
+    top[3], top[v - 2] = INF, INF
+    for t in (INF, 1e300):
+        t = torch.full((4,), t, dtype=torch.float64, device=DEV)
+        assert ops.sample(row.expand(4, v), u, temperature=t).tolist() == want
+        assert ops.sample(top.expand(4, v), u, temperature=t).tolist() == [3, 3, v - 2, v - 2]
+        assert ops.sample(top.expand(4, v), u, temperature=t, top_k=2,
+                          top_p=0.9).tolist() == [3, 3, v - 2, v - 2]
+
+
+@gpu
+@pytest.mark.parametrize("form,dtype,v", SAMPLE_FORMS)
+@pytest.mark.parametrize("t", [1e-10, 1e-30, 5e-324])
+def test_sample_near_zero_temperature_beside_nan(form, dtype, v, t):
+    row = _finite_row(dtype, v, 302)
+    row[_every_third(v, 70, 5)] = NAN
+    top = _every_third(v, 5, v // 2)
+    row[top] = 60.0
+    for settings in (dict(), dict(top_k=9), dict(top_p=0.999), dict(min_p=0.5)):
+        got = ops.sample(row.expand(5, v), _mids(5), temperature=t, **settings)
+        assert got.tolist() == top, settings
