@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from lambdipy_amd import ops
-from tests.test_decode_ops_gpu import DEV, _randn, gpu
+from tests.test_decode_ops_gpu import DEV, TYPES, _gen, _randn, _sample64, _uniform, gpu
 
 INF, NAN = float("inf"), float("nan")
 
@@ -89,3 +89,51 @@ def test_sample_near_zero_temperature_beside_nan(form, dtype, v, t):
     for settings in (dict(), dict(top_k=9), dict(top_p=0.999), dict(min_p=0.5)):
         got = ops.sample(row.expand(5, v), _mids(5), temperature=t, **settings)
         assert got.tolist() == top, settings
+
+
+# ---- sampling: rows that are mostly masked -----------------------------------
+
+# A weight is held in steps of 2^-45 and off by half of one and by 2^-44 of
+# itself, so a running weight over V logits (in all 1 or more) by less than
+# V * 2^-46 + 2^-44 of the row's; a border that is nearer than twice that may
+# be decided either way.
+def _near_of(v):
+    return 2 * (v * 2.0 ** -46 + 2.0 ** -44)
+
+
+def _masked_rows(dtype, mask, v, seed):
+    """Rows of which a part, nearly all or all is at one value."""
+    x = _randn((6, v), seed, dtype, 2.0)
+    if mask == 0.0:
+        x = x.abs()  # the masked are the lowest
+    m = torch.finfo(dtype).min if mask == "lowest" else mask
+    there = torch.rand((6, v), generator=_gen(seed + 1)).to(DEV)
+    x[0] = torch.where(there[0] < 0.9, m, x[0])
+    x[1] = torch.where(there[1] < 0.5, m, x[1])
+    x[2] = torch.where(there[2] < 0.9999, m, x[2])
+    x[3] = m
+    x[4, 17:] = m
+    x[5] = torch.where(there[5] < 0.6, m, -m if mask == 0.0 else x[5])
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("mask", [-INF, "lowest", -1e4, 0.0, -0.0, NAN])
+@pytest.mark.parametrize("settings", [
+    {}, dict(top_k=50), dict(top_k=120000), dict(top_p=0.9), dict(min_p=0.05),
+    dict(top_k=40, top_p=0.5, temperature=0.7), dict(temperature=0.0)])
+@pytest.mark.parametrize("v", [5003, 131075])
+def test_sample_tokens_of_rows_that_are_mostly_masked(dtype, mask, settings, v):
+    x = _masked_rows(dtype, mask, v, 310)
+    u = _uniform(6, 312)
+    got = ops.sample(x, u, **settings).cpu()
+    want, near = _sample64(x, u, **settings)
+    # Where all that can be kept is equal, every weight is 1 on both sides, its
+    # sums are whole numbers, and the borders are the same products rounded the
+    # same (times 2^45): nothing is near.
+    k = settings.get("top_k", 0) or v
+    top = x.float().nan_to_num(nan=-INF, posinf=INF, neginf=-INF).topk(min(k, v), dim=1).values
+    sure = (near > _near_of(v)) | (top == top[:, :1]).all(dim=1).cpu()
+    assert int(sure.sum()) >= 5  # one row may lie at a border by chance
+    assert got[sure].tolist() == want[sure].tolist()
