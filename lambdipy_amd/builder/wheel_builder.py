@@ -12,8 +12,8 @@ runtime, so a native recipe's artifact is built directly:
   is copied next to it.
 
 Artifact reuse: the in-tree .so acts as the content-addressed cache entry
-(rebuilt only when sources change — setup.py/ninja dependency tracking), the
-analog of lambdipy's prebuilt-artifact reuse (SURVEY.md §5 checkpoint row).
+(rebuilt only when sources or compiler flags change — setup.py/ninja
+dependency tracking, builder/flags.py), the analog of lambdipy's prebuilt-artifact reuse (SURVEY.md §5 checkpoint row).
 """
 
 from __future__ import annotations
@@ -27,6 +27,7 @@ from typing import Optional
 from ..recipes import BuildRecipe
 from ..resolver import ResolvedDep
 from ..utils.log import get_logger
+from . import flags
 
 log = get_logger("builder")
 
@@ -41,10 +42,6 @@ def ops_extension_path() -> Optional[str]:
     return hits[0] if hits else None
 
 
-# Device code is compiled without packed f32 instructions: some forms of
-# v_pk_{add,mul,fma}_f32 gave wrong results on MI355X (setup.py has the same).
-NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
 HSACO_PATH = os.path.join(OPS_DIR, "standalone_gfx950.hsaco")
 HSACO_SRC = os.path.join(OPS_DIR, "csrc", "standalone.hip")
 
@@ -52,20 +49,20 @@ HSACO_SRC = os.path.join(OPS_DIR, "csrc", "standalone.hip")
 def ensure_standalone_hsaco(allow_build: bool = True) -> str:
     """AOT code object for the torch-free runtime (hipcc --genco, gfx950).
 
-    Rebuilt when missing or older than its source; ships in-tree (the .hsaco
-    is git-ignored but travels with snapshots / into recipe wheels)."""
-    if os.path.exists(HSACO_PATH) and (
+    Rebuilt when missing, older than its source or built with other flags;
+    ships in-tree (the .hsaco is git-ignored but travels with snapshots / into
+    recipe wheels)."""
+    args = ["--genco", "--offload-arch=gfx950", "-O3", *flags.NO_PACKED_F32]
+    if flags.built_with(HSACO_PATH, args) and (
         os.path.getmtime(HSACO_PATH) >= os.path.getmtime(HSACO_SRC)
     ):
         return HSACO_PATH
     if not allow_build:
-        raise RuntimeError("standalone hsaco missing and allow_build=False")
+        raise RuntimeError("standalone hsaco missing or stale and allow_build=False")
     log.info("building standalone gfx950 code object (hipcc --genco)...")
-    subprocess.run(
-        ["hipcc", "--genco", "--offload-arch=gfx950", "-O3", *NO_PACKED_F32,
-         HSACO_SRC, "-o", HSACO_PATH],
-        check=True,
-    )
+    flags.forget(HSACO_PATH)
+    subprocess.run(["hipcc", *args, HSACO_SRC, "-o", HSACO_PATH], check=True)
+    flags.record(HSACO_PATH, args)
     return HSACO_PATH
 
 
@@ -83,8 +80,8 @@ def ensure_nn_lib(allow_build: bool = True) -> str:
     extension uses (ops/csrc/*.hip) plus the C API (nn_capi.cpp) — one
     kernel code base, two front ends. AOT gfx950, ships in-tree (git-ignored
     .so travels with snapshots / into recipe wheels). Parallel per-file
-    compiles with mtime-based reuse; objects cached next to the sources in
-    ops/csrc/.nnobj/."""
+    compiles, reused by mtime and flags; objects cached next to the sources
+    in ops/csrc/.nnobj/."""
     csrc = os.path.join(OPS_DIR, "csrc")
     sources = sorted(
         os.path.join(csrc, f)
@@ -95,51 +92,58 @@ def ensure_nn_lib(allow_build: bool = True) -> str:
     )
     headers = [os.path.join(csrc, h) for h in ("kernels.h", "lpx_common.h")]
     hdr_mtime = max(os.path.getmtime(h) for h in headers)
-    if os.path.exists(NN_LIB_PATH):
+    compile_args = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
+                    "-fvisibility=hidden", *flags.NO_PACKED_F32]
+    # the library's own: also which sources are in it
+    lib_args = compile_args + [os.path.basename(s) for s in sources]
+    if flags.built_with(NN_LIB_PATH, lib_args):
         lib_m = os.path.getmtime(NN_LIB_PATH)
         if lib_m >= hdr_mtime and all(
             lib_m >= os.path.getmtime(s) for s in sources
         ):
             return NN_LIB_PATH
     if not allow_build:
-        raise RuntimeError("liblpx_nn missing and allow_build=False")
+        raise RuntimeError("liblpx_nn missing or stale and allow_build=False")
     log.info("building liblpx_nn_gfx950.so (hipcc, %d sources)...", len(sources))
     objdir = os.path.join(csrc, ".nnobj")
     os.makedirs(objdir, exist_ok=True)
-    flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
-             "-fvisibility=hidden", "-I", csrc, *NO_PACKED_F32]
     procs = []
     objs = []
     for s in sources:
         o = os.path.join(objdir, os.path.basename(s) + ".o")
         objs.append(o)
-        if os.path.exists(o) and os.path.getmtime(o) >= max(
+        if flags.built_with(o, compile_args) and os.path.getmtime(o) >= max(
             os.path.getmtime(s), hdr_mtime
         ):
             continue
-        procs.append((s, subprocess.Popen(
-            ["hipcc", "-c", s, "-o", o] + flags,
+        flags.forget(o)
+        procs.append((s, o, subprocess.Popen(
+            ["hipcc", "-c", s, "-o", o, "-I", csrc, *compile_args],
             stdout=subprocess.PIPE, stderr=subprocess.PIPE)))
-    for s, p in procs:
+    for s, o, p in procs:
         out, err = p.communicate()
         if p.returncode != 0:
             raise RuntimeError(
                 f"hipcc failed on {s}:\n{err.decode()[-4000:]}")
+        flags.record(o, compile_args)
+    flags.forget(NN_LIB_PATH)
     subprocess.run(
         ["hipcc", "-shared", "-fPIC", "--offload-arch=gfx950",
          "-o", NN_LIB_PATH] + objs,
         check=True,
     )
+    flags.record(NN_LIB_PATH, lib_args)
     return NN_LIB_PATH
 
 
 def ensure_ops_extension(allow_build: bool = True) -> str:
-    """Return the built extension path, building it in-tree if needed."""
+    """Return the built extension path, building it in-tree if it is missing
+    or was built with other flags."""
     p = ops_extension_path()
-    if p:
+    if p and flags.built_with(p, flags.OPS_HIP):
         return p
     if not allow_build:
-        raise RuntimeError("ops extension not built and allow_build=False")
+        raise RuntimeError("ops extension not built as it is now and allow_build=False")
     log.info("building gfx950 ops extension (hipcc AOT)...")
     env = dict(os.environ, PYTORCH_ROCM_ARCH="gfx950")
     subprocess.run(

@@ -8,6 +8,7 @@ repo tree and travels to the GPU box with the source snapshot.
 """
 
 import os
+import runpy
 
 from setuptools import setup
 
@@ -17,6 +18,7 @@ from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E40
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "lambdipy_amd", "ops", "csrc")
+FLAGS = runpy.run_path(os.path.join(ROOT, "lambdipy_amd", "builder", "flags.py"))
 
 sources = [
     os.path.join(CSRC, f)
@@ -25,6 +27,22 @@ sources = [
     and f != "standalone.hip"  # --genco code object, built by the builder
     and f != "nn_capi.cpp"  # liblpx_nn C API, built by builder.ensure_nn_lib
 ]
+
+
+
+class BuildOps(BuildExtension):
+    """Builds again, too, what was built with other flags."""
+
+    def run(self):
+        paths = [self.get_ext_fullpath(ext.name) for ext in self.extensions]
+        for path in paths:
+            if not FLAGS["built_with"](path, FLAGS["OPS_HIP"]):
+                self.force = True
+                FLAGS["forget"](path)
+        super().run()
+        for path in paths:
+            FLAGS["record"](path, FLAGS["OPS_HIP"])
+
 
 setup(
     name="lambdipy-amd",
@@ -47,15 +65,10 @@ setup(
         CUDAExtension(
             name="lambdipy_amd.ops._lpx_ops",
             sources=sources,
-            extra_compile_args={
-                "cxx": ["-O3", "-std=c++17"],
-                # device code without packed f32 instructions: some forms of
-                # v_pk_{add,mul,fma}_f32 gave wrong results on MI355X
-                "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
-                         "-Xclang", "-packed-fp32-ops"],
-            },
+            depends=[os.path.join(CSRC, h) for h in ("kernels.h", "lpx_common.h")],
+            extra_compile_args={"cxx": FLAGS["OPS_CXX"], "nvcc": FLAGS["OPS_HIP"]},
         )
     ],
-    cmdclass={"build_ext": BuildExtension},
+    cmdclass={"build_ext": BuildOps},
     entry_points={"console_scripts": ["lpx = lambdipy_amd.cli:main"]},
 )
