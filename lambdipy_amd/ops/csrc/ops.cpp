@@ -793,15 +793,6 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& l
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
-// A dense part of an allocation.
-at::Tensor part_of(const at::Tensor& block, int64_t offset, at::IntArrayRef sizes) {
-  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(block.storage()),
-                                                    block.key_set(), block.dtype());
-  t.unsafeGetTensorImpl()->set_storage_offset(offset);
-  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-  return t;
-}
-
 void inference_only(const at::Tensor& t, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
               " has no backward pass: call it under torch.no_grad() or on detached tensors");
@@ -874,10 +865,8 @@ py::object rmsnorm_mx(const at::Tensor& x, const at::Tensor& weight,
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) % 64 == 0, "rmsnorm_mx expects x [..., K%64==0]");
   NormCall c = norm_call(x, weight, residual, eps, "rmsnorm_mx");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-  // payload and scales, which go together, as one allocation
-  const int64_t tiles = (c.K + 127) / 128, bytes = ((int64_t)c.R * c.K + 255) / 256 * 256;
-  const auto block = fresh({bytes + tiles * c.R * 4}, at::kByte, x);
-  const auto q = part_of(block, 0, {c.R, c.K}), sc = part_of(block, bytes, {tiles, c.R, 4});
+  const auto q = fresh({c.R, c.K}, at::kByte, x);
+  const auto sc = fresh({(c.K + 127) / 128, c.R, 4}, at::kByte, x);
   check_hip(lpx::rmsnorm_mx(c.type, c.x.data_ptr(), c.x.stride(0),
                             c.r.defined() ? c.r.data_ptr() : nullptr,
                             c.r.defined() ? c.r.stride(0) : 0, c.w.data_ptr(),

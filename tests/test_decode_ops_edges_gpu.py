@@ -9,6 +9,19 @@ from tests.test_decode_ops_gpu import DEV, TYPES, _gen, _randn, _sample64, _unif
 INF, NAN = float("inf"), float("nan")
 
 
+# ---- residual + RMS norm -----------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("rows,k", [(1, 64), (5, 4096)])
+def test_rmsnorm_mx_results_have_memory_of_their_own(rows, k):
+    # keeping or saving one of them does not keep or save the others
+    x = _randn((rows, k), 290, torch.bfloat16)
+    out = ops.rmsnorm_mx(x, _randn((k,), 291), residual=x)
+    assert [t.untyped_storage().nbytes() for t in out] == [t.nbytes for t in out]
+    assert len({t.untyped_storage().data_ptr() for t in out}) == 3
+    assert all(t.storage_offset() == 0 and t.is_contiguous() for t in out)
+
+
 # ---- sampling: NaN beside infinities ----------------------------------------
 
 # how a row is sampled: f32 in one workgroup or as chunks; 16 bits by the count
