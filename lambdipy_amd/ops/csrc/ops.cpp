@@ -796,6 +796,9 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& l
 void inference_only(const at::Tensor& t, const char* what) {
   TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
               " has no backward pass: call it under torch.no_grad() or on detached tensors");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+                t._fw_grad(0).defined()),
+              what, " has no forward-mode derivative: the tangent would be lost");
 }
 
 // Rows of a 2-D view whose last axis is dense; rows may be further apart.

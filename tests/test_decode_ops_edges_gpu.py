@@ -2,9 +2,10 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from lambdipy_amd import ops
-from tests.test_decode_ops_gpu import DEV, TYPES, _gen, _randn, _sample64, _uniform, gpu
+from tests.test_decode_ops_gpu import DEV, TYPES, _gen, _randn, _sample64, _uniform, built, gpu
 
 INF, NAN = float("inf"), float("nan")
 
@@ -20,6 +21,31 @@ def test_rmsnorm_mx_results_have_memory_of_their_own(rows, k):
     assert [t.untyped_storage().nbytes() for t in out] == [t.nbytes for t in out]
     assert len({t.untyped_storage().data_ptr() for t in out}) == 3
     assert all(t.storage_offset() == 0 and t.is_contiguous() for t in out)
+
+
+@built
+def test_a_tangent_is_refused_and_not_lost():
+    x, w = torch.zeros(2, 64), torch.ones(64)
+    w4, sw = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(1, 8, 4, dtype=torch.uint8)
+
+    def refused(why, *calls):
+        for call in calls:
+            with pytest.raises(RuntimeError, match=why):
+                call()
+
+    with fwAD.dual_level(), torch.no_grad():
+        dx, dw = fwAD.make_dual(x, x), fwAD.make_dual(w, w)
+        db = fwAD.make_dual(x.bfloat16(), x.bfloat16())
+        refused("forward-mode", lambda: ops.gemv_w4(db, w4, sw))
+        for op in (ops.rmsnorm, ops.rmsnorm_mx):
+            refused("forward-mode", lambda: op(dx, w), lambda: op(x, dw),
+                    lambda: op(x, w, residual=dx))
+            # what carries none, or where none is asked for, goes on to the device
+            refused("on the ROCm device", lambda: op(fwAD.unpack_dual(dx).primal, w),
+                    lambda: op(x, w))
+            with fwAD._set_fwd_grad_enabled(False):
+                refused("on the ROCm device", lambda: op(dx, w))
+    refused("forward-mode", lambda: torch.func.jvp(lambda v: ops.rmsnorm(v, w), (x,), (x,)))
 
 
 # ---- sampling: NaN beside infinities ----------------------------------------
