@@ -158,7 +158,7 @@ def gemv_w4(x: torch.Tensor, Bt4: torch.Tensor, sB: torch.Tensor,
     weights (weight-only quantisation: x is not rounded).
 
     x [..., K] bf16 or fp16 (rows may be strided), Bt4 [N, K/2] and sB from
-    quantize_mx_fp4, any N, K%64==0. Returns [..., N] f32, or bf16. Made for
+    quantize_mx_fp4, any N below 2^28, K%64==0. Returns [..., N] f32, or bf16. Made for
     one to 64 rows, where reading the weights is all the time; more rows are
     taken 64 at a time. Sums in f32, in a fixed order."""
     return require_extension().gemv_w4(x, Bt4, sB, bf16_out)

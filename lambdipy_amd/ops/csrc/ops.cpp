@@ -892,7 +892,8 @@ void check_w4(const at::Tensor& w, const at::Tensor& sw, int64_t K, const char* 
               ": scale shapes must be [ceil(K/128), rows, 4] (tile-major)");
   TORCH_CHECK(w.is_contiguous() && sw.is_contiguous(), what,
               ": weights and scales must be contiguous");
-  TORCH_CHECK(K <= (1 << 24) && w.size(0) <= (1 << 30), what, ": too large");
+  // (a grid's threads are fewer than 2^32: 16 at most for a row of weights)
+  TORCH_CHECK(K <= (1 << 24) && w.size(0) <= (1 << 28) - 64, what, ": too large");
 }
 
 at::Tensor gemv_w4(const at::Tensor& x, const at::Tensor& Bt4, const at::Tensor& sB,

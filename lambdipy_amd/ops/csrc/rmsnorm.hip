@@ -19,6 +19,8 @@
 // the code for widths that are no multiple of 8; a copy of that size in torch
 // reaches 4.9.
 
+#include <algorithm>
+
 #include "lpx_common.h"
 #include "kernels.h"
 
@@ -148,6 +150,7 @@ struct NormArgs {
   unsigned char* sc;
   long x_stride, res_stride;  // elements
   int R, K;
+  int first;  // row of the launch's first
   float eps;
   bool weight_f32;
 };
@@ -188,7 +191,7 @@ __device__ __forceinline__ float square_sum(f32x8 h) {
 template <typename T, bool MX, bool WHOLE>
 __global__ __launch_bounds__(256) void rmsnorm_short_kernel(NormArgs a, int lanes) {
   const int rows = 256 / lanes;
-  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x) * rows +
+  const int row = a.first + (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x) * rows +
                   (int)threadIdx.x / lanes;
   const int c = row < a.R ? (int)threadIdx.x % lanes * 8 : a.K;
   f32x8 h = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(256) void rmsnorm_short_kernel(NormArgs a, int lane
 template <typename T, bool MX, bool WHOLE, int STEPS>
 __global__ __launch_bounds__(1024) void rmsnorm_kernel(NormArgs a) {
   // neighbouring rows on one XCD: their scale bytes share lines of its L2
-  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
+  const int row = a.first + (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
   f32x8 h[STEPS];
   float s = 0.f;
 #pragma unroll
@@ -221,7 +224,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_kernel(NormArgs a) {
 // Longer rows: read a second time (the first pass left them in the caches).
 template <typename T, bool MX, bool WHOLE>
 __global__ __launch_bounds__(1024) void rmsnorm_long_kernel(NormArgs a) {
-  const int row = (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
+  const int row = a.first + (int)lpx_xcd_swizzle(blockIdx.x, gridDim.x);
   const int steps = (a.K + 8191) / 8192;
   float s = 0.f;
   for (int i = 0; i < steps; ++i) {
@@ -252,29 +255,39 @@ bool two_steps(int R, int waves) {
   return R <= (waves > 8 ? 2 * slots : slots + slots / 4);
 }
 
+// `each` rows to a workgroup of `threads`. A grid's threads are counted in 32
+// bits, so that very many rows take more than one.
+template <typename Kernel, typename... More>
+hipError_t launch_rows(Kernel kernel, NormArgs a, int each, int threads,
+                       hipStream_t stream, More... more) {
+  const int most = 0x7fffffff / threads;  // workgroups
+  for (long first = 0; first < a.R; first += (long)most * each) {
+    const long left = (a.R - first + each - 1) / each;
+    const dim3 grid((unsigned)std::min<long>(left, most)), block((unsigned)threads);
+    a.first = (int)first;
+    kernel<<<grid, block, 0, stream>>>(a, more...);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <typename T, bool MX, bool WHOLE>
 hipError_t launch(const NormArgs& a, hipStream_t stream) {
   const int threads = (a.K + 7) / 8;
   if (threads <= 64) {
     int lanes = 8;
     while (lanes < threads) lanes *= 2;
-    const int rows = 256 / lanes;
-    rmsnorm_short_kernel<T, MX, WHOLE>
-        <<<dim3((unsigned)((a.R + rows - 1) / rows)), dim3(256), 0, stream>>>(a, lanes);
-    return hipGetLastError();
+    return launch_rows(rmsnorm_short_kernel<T, MX, WHOLE>, a, 256 / lanes, 256, stream, lanes);
   }
   const int waves = (threads + 63) / 64;
-  const dim3 grid((unsigned)a.R), block((unsigned)waves * 64), most(1024);
   if (threads <= 1024 && two_steps<T, WHOLE>(a.R, waves))
-    rmsnorm_kernel<T, MX, WHOLE, 2>
-        <<<grid, dim3((unsigned)(waves + 1) / 2 * 64), 0, stream>>>(a);
-  else if (threads <= 1024)
-    rmsnorm_kernel<T, MX, WHOLE, 1><<<grid, block, 0, stream>>>(a);
-  else if (threads <= 2048)
-    rmsnorm_kernel<T, MX, WHOLE, 2><<<grid, most, 0, stream>>>(a);
-  else
-    rmsnorm_long_kernel<T, MX, WHOLE><<<grid, most, 0, stream>>>(a);
-  return hipGetLastError();
+    return launch_rows(rmsnorm_kernel<T, MX, WHOLE, 2>, a, 1, (waves + 1) / 2 * 64, stream);
+  if (threads <= 1024)
+    return launch_rows(rmsnorm_kernel<T, MX, WHOLE, 1>, a, 1, waves * 64, stream);
+  if (threads <= 2048)
+    return launch_rows(rmsnorm_kernel<T, MX, WHOLE, 2>, a, 1, 1024, stream);
+  return launch_rows(rmsnorm_long_kernel<T, MX, WHOLE>, a, 1, 1024, stream);
 }
 
 template <typename T, bool MX>
@@ -303,7 +316,7 @@ hipError_t rmsnorm(ActType t, const void* x, long x_stride, const void* res,
                    float eps, void* h, void* y, int R, int K,
                    hipStream_t stream) {
   return by_type<false>(t, NormArgs{x, res, weight, h, y, nullptr, x_stride,
-                                    res_stride, R, K, eps, weight_f32},
+                                    res_stride, R, K, 0, eps, weight_f32},
                         stream);
 }
 
@@ -312,7 +325,7 @@ hipError_t rmsnorm_mx(ActType t, const void* x, long x_stride, const void* res,
                       float eps, void* h, unsigned char* q, unsigned char* sc,
                       int R, int K, hipStream_t stream) {
   return by_type<true>(t, NormArgs{x, res, weight, h, q, sc, x_stride,
-                                   res_stride, R, K, eps, weight_f32},
+                                   res_stride, R, K, 0, eps, weight_f32},
                        stream);
 }
 

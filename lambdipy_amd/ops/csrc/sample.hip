@@ -1376,6 +1376,27 @@ hipError_t launch(const SampleArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+hipError_t launch_type(ActType t, const SampleArgs& a, hipStream_t stream) {
+  switch (t) {
+    case ActType::bf16: return launch<__bf16>(a, stream);
+    case ActType::f16: return launch<_Float16>(a, stream);
+    case ActType::f32: return launch<float>(a, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+// A setting's values from row `first` on.
+SampleParam from_row(SampleParam p, long first) {
+  const int size = p.kind == SampleParam::f32 || p.kind == SampleParam::i32 ? 4 : 8;
+  if (p.kind != SampleParam::value_) p.ptr = static_cast<const char*>(p.ptr) + first * size;
+  return p;
+}
+
+// Rows to a launch, whose threads are counted in 32 bits: a row takes 1024 in
+// one workgroup, or in chunks no more (they are 4096 logits at least, and more
+// than two a row only where there are few rows).
+constexpr int MOST_ROWS = 1 << 21;
+
 struct Plan {
   int chunk, chunks;
   size_t bins_at, scales_at, bytes;
@@ -1385,6 +1406,7 @@ Plan plan_of(ActType t, int rows, int vocab) {
   // At least 4096 logits a chunk; more where there are chunks enough for the
   // chip without that, so that fewer histograms are written.
   Plan p{};
+  if (rows > MOST_ROWS) rows = MOST_ROWS;
   if (t != ActType::f32 || vocab <= (rows >= MANY ? WHOLE_MANY : WHOLE)) return p;
   const long want = ((long)rows * vocab + 2047) / 2048;
   p.chunk = want <= 4096 ? 4096 : (int)(((want < vocab ? want : vocab) + 511) / 512 * 512);
@@ -1409,23 +1431,28 @@ hipError_t sample(ActType t, const void* logits, long stride, int rows,
   if (vocab <= 0) return hipErrorInvalidValue;
   if (t != ActType::f32 && vocab > SAMPLE_MOST_16) return hipErrorInvalidValue;
   const Plan p = plan_of(t, rows, vocab);
-  if ((int64_t)rows * p.chunks >= (int64_t(1) << 31)) return hipErrorInvalidValue;
   int shift = 45;  // sums of `vocab` weights stay below 2^62
   while (vocab > (int64_t(1) << (62 - shift))) --shift;
   char* const work = static_cast<char*>(workspace);
-  SampleArgs a{logits, stride, rows, vocab, p.chunk, p.chunks, shift,
+  const SampleArgs a{logits, stride, rows, vocab, p.chunk, p.chunks, shift,
                temperature, top_k, top_p, min_p, u,
                reinterpret_cast<ChunkMax*>(work),
                reinterpret_cast<ChunkBins*>(work + p.bins_at),
                reinterpret_cast<RowScale*>(work + p.scales_at),
                temperature.kind != SampleParam::value_ || temperature.value > 0,
                token};
-  switch (t) {
-    case ActType::bf16: return launch<__bf16>(a, stream);
-    case ActType::f16: return launch<_Float16>(a, stream);
-    case ActType::f32: return launch<float>(a, stream);
+  // one launch after the other, in the same workspace
+  for (long first = 0; first < rows; first += MOST_ROWS) {
+    SampleArgs now = a;
+    now.logits = static_cast<const char*>(logits) + first * stride * (t == ActType::f32 ? 4 : 2);
+    now.rows = (int)(rows - first < MOST_ROWS ? rows - first : MOST_ROWS);
+    for (SampleParam* p : {&now.temperature, &now.top_k, &now.top_p, &now.min_p, &now.u})
+      *p = from_row(*p, first);
+    now.token = token + first;
+    const hipError_t e = launch_type(t, now, stream);
+    if (e != hipSuccess) return e;
   }
-  return hipErrorInvalidValue;
+  return hipSuccess;
 }
 
 }  // namespace lpx

@@ -48,6 +48,74 @@ def test_a_tangent_is_refused_and_not_lost():
     refused("forward-mode", lambda: torch.func.jvp(lambda v: ops.rmsnorm(v, w), (x,), (x,)))
 
 
+# ---- more rows than one launch has threads for -------------------------------
+# A grid holds fewer than 2^32 threads.
+
+@gpu
+@pytest.mark.parametrize("dtype,k,rows", [
+    (torch.float16, 1, 2 ** 29 + 5),     # eight threads a row
+    (torch.bfloat16, 520, 2 ** 25 + 3)])  # 128
+def test_rmsnorm_past_a_grid(dtype, k, rows):
+    some = _randn((7, k), 320, dtype)
+    w = _randn((k,), 321, dtype)
+    want = ops.rmsnorm(some, w)
+    if k == 1:
+        y = ops.rmsnorm(some.repeat(rows // 7 + 1, 1)[:rows], w)
+        whole = rows // 7 * 7
+        assert bool((y[:whole].view(-1, 7) == want.view(1, 7)).all())
+        assert torch.equal(y[whole:], want[:rows - whole])
+    else:  # one row for all, so that only the result takes memory
+        y = ops.rmsnorm(some[:1].expand(rows, k), w)
+        for at in range(0, rows, 2 ** 22):
+            assert bool((y[at:at + 2 ** 22] == want[:1]).all())
+
+
+@gpu
+def test_rmsnorm_mx_past_a_grid():
+    k, rows = 576, 2 ** 25 + 3
+    x, w = _randn((1, k), 322, torch.bfloat16), _randn((k,), 323)
+    q1, sc1 = ops.rmsnorm_mx(x, w)
+    q, sc = ops.rmsnorm_mx(x.expand(rows, k), w)
+    for at in range(0, rows, 2 ** 22):
+        assert bool((q[at:at + 2 ** 22] == q1).all())
+        assert bool((sc[:, at:at + 2 ** 22] == sc1).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("of_each_row", [False, True])
+def test_sample_past_a_grid(dtype, of_each_row):
+    rows = 2 ** 22 + 5  # 1024 threads each
+    w = torch.tensor([0.125, 0.5, 0.0625, 0.3125], dtype=torch.float64)
+    logits = w.log().to(dtype).to(DEV).expand(rows, 4)
+    u = _uniform(rows, 324)
+    settings = dict(temperature=0.0)
+    want = torch.ones(rows, dtype=torch.int64)
+    if of_each_row:
+        settings = dict(temperature=torch.ones(rows, device=DEV),
+                        top_k=torch.arange(rows, dtype=torch.int32, device=DEV) % 4 + 1)
+        # in falling order: 1, 3, 0, 2
+        c = torch.exp(logits[0].double().cpu()[[1, 3, 0, 2]]).cumsum(0)
+        draw = u.double().cpu() * c[torch.arange(rows) % 4]
+        want = torch.tensor([1, 3, 0, 2])[(c.unsqueeze(0) <= draw.unsqueeze(1)).sum(1)]
+        sure = ((c.unsqueeze(0) - draw.unsqueeze(1)).abs() > 1e-12).all(dim=1)
+    got = ops.sample(logits, u, **settings).cpu()
+    differ = got != want
+    assert not bool((differ & sure if of_each_row else differ).any())
+
+
+@built
+def test_gemv_4bit_refuses_more_weights_than_a_grid_has_threads_for():
+    n = 2 ** 28 - 63
+    w4 = torch.empty(n, 32, dtype=torch.uint8, device="meta")
+    sw = torch.empty(1, n, 4, dtype=torch.uint8, device="meta")
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.gemv_w4(torch.zeros(1, 64, dtype=torch.bfloat16), w4, sw)
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.gemv_mx_w4(torch.zeros(1, 64, dtype=torch.uint8),
+                       torch.zeros(1, 1, 4, dtype=torch.uint8), w4, sw)
+
+
 # ---- sampling: NaN beside infinities ----------------------------------------
 
 # how a row is sampled: f32 in one workgroup or as chunks; 16 bits by the count
