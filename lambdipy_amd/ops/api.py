@@ -158,18 +158,21 @@ def gemv_w4(x: torch.Tensor, Bt4: torch.Tensor, sB: torch.Tensor,
     weights (weight-only quantisation: x is not rounded).
 
     x [..., K] bf16 or fp16 (rows may be strided), Bt4 [N, K/2] and sB from
-    quantize_mx_fp4, any N below 2^28, K%64==0. Returns [..., N] f32, or bf16. Made for
-    one to 64 rows, where reading the weights is all the time; more rows are
-    taken 64 at a time. Sums in f32, in a fixed order."""
+    quantize_mx_fp4, any N below 2^28, K%64==0. Returns [..., N] f32, or bf16.
+    Made for one to 64 rows, where reading the weights is all the time; more
+    rows are taken 64 at a time (32 of fp16, fewer where N is small). Weights
+    are exact for scale bytes up to 252 (6 * 2^125); 255 is NaN. Sums in f32,
+    in a fixed order."""
     return require_extension().gemv_w4(x, Bt4, sB, bf16_out)
 
 
 def gemv_mx_w4(A: torch.Tensor, sA: torch.Tensor, Bt4: torch.Tensor,
                sB: torch.Tensor, bf16_out: bool = False) -> torch.Tensor:
     """gemm_mx_w4 for a few rows: A [M, K] and sA from quantize_mx or
-    rmsnorm_mx, weights as for gemv_w4, any M and N. Both sides' values are
-    exact and their products summed in f32 (gemm_mx_w4's scaled MFMA holds
-    its inner sums less exactly)."""
+    rmsnorm_mx, weights and N as for gemv_w4, any M. Both sides' values are
+    exact (of A for scale bytes 3 to 246: under 2^-133 bits are lost, past
+    448 * 2^119 is infinite) and their products summed in f32 (gemm_mx_w4's
+    scaled MFMA holds its inner sums less exactly)."""
     return require_extension().gemv_mx_w4(A, sA, Bt4, sB, bf16_out)
 
 

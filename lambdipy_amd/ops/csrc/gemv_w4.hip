@@ -5,7 +5,9 @@
 // x in bf16 or fp16, or MX e4m3 with scales of its own. What has to move is
 // the weights (0.53 B an element). The products are taken by the 16-bit MFMA
 // with f32 sums: e2m1 and e4m3 values times their power of two are exact in
-// bf16, and so is every product in f32. (The scaled f8f6f4 MFMA would take
+// bf16 (scale bytes of weights up to 252, of activations 3 to 246: more is
+// infinite, less loses what is under 2^-133; 255 is NaN), and so is every
+// product in f32. (The scaled f8f6f4 MFMA would take
 // the bytes as they are, but does not hold its inner sums to f32: 2.7e-5 off
 // over K = 512.)
 //
@@ -63,6 +65,12 @@ __device__ __forceinline__ unsigned load4(const unsigned char* p) {
 // Byte i of a scale word as 2^(byte - 127); 2^-127 is an f32 subnormal.
 __device__ __forceinline__ float scale_of(unsigned word, int i) {
   return __uint_as_float(max(((word >> (8 * i)) & 255u) << 23, 0x400000u));
+}
+
+// Of a scale that goes onto a sum: 255 is NaN. (The conversions take the
+// infinity of scale_of as that.)
+__device__ __forceinline__ float nan_or_scale_of(unsigned word, int i) {
+  return ((word >> (8 * i)) & 255u) == 255u ? __builtin_nanf("") : scale_of(word, i);
 }
 
 // 8 e2m1 (one word) times s -> bf16
@@ -303,7 +311,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemv_w4_kernel(W4Args a) {
             const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                 __builtin_bit_cast(nf16x8, x), __builtin_bit_cast(nf16x8, b[t]),
                 f32x4{0, 0, 0, 0}, 0, 0, 0);
-            const float sc = scale_of(q.sw[t], j);
+            const float sc = nan_or_scale_of(q.sw[t], j);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               acc[i][t][r] = __builtin_fmaf(p[r], sc, acc[i][t][r]);

@@ -5,7 +5,8 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 from lambdipy_amd import ops
-from tests.test_decode_ops_gpu import DEV, TYPES, _gen, _randn, _sample64, _uniform, built, gpu
+from tests.test_decode_ops_gpu import (DEV, TYPES, _fp4_values, _gen, _mx_values, _randn,
+                                       _sample64, _uniform, _weights, built, gpu)
 
 INF, NAN = float("inf"), float("nan")
 
@@ -46,6 +47,73 @@ def test_a_tangent_is_refused_and_not_lost():
             with fwAD._set_fwd_grad_enabled(False):
                 refused("on the ROCm device", lambda: op(dx, w))
     refused("forward-mode", lambda: torch.func.jvp(lambda v: ops.rmsnorm(v, w), (x,), (x,)))
+
+
+# ---- 4-bit weights: scales at their ends -------------------------------------
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+@pytest.mark.parametrize("byte", [0, 1, 2, 3, 4, 127, 250, 251, 252])
+def test_gemv_4bit_weights_are_exact_at_scale(act, byte):
+    # one-hot rows give back the dequantised weights, and with x shrunk or
+    # grown they give the same weights at the other end of the exponents
+    n, k = 40, 64
+    w4, sw = _weights(n, k, 330)
+    sw.fill_(byte)
+    want = _fp4_values(w4, sw).t()
+    eye = torch.eye(k, device=DEV)
+    if act == "mx":
+        got = ops.gemv_mx_w4(*ops.quantize_mx(eye), w4, sw)
+    else:
+        got = ops.gemv_w4(eye.to(torch.bfloat16 if act == "bf16" else torch.float16), w4, sw)
+    assert torch.equal(got.double(), want)
+    if act == "bf16":
+        s = 2.0 ** min(max(127 - byte, -120), 120)
+        assert torch.equal(ops.gemv_w4((eye * s).bfloat16(), w4, sw).double(), want * s)
+
+
+@gpu
+@pytest.mark.parametrize("byte", [3, 4, 9, 10, 127, 245, 246])
+def test_gemv_4bit_activations_are_exact_at_scale(byte):
+    # every finite e4m3 value at that scale, by a weight that brings it back
+    v = torch.tensor([i for i in range(256) if i & 127 != 127], dtype=torch.uint8, device=DEV)
+    q = torch.zeros(len(v), 64, dtype=torch.uint8, device=DEV)
+    q[:, 0] = v
+    sq = torch.full((1, len(v), 4), byte, dtype=torch.uint8, device=DEV)
+    w4 = torch.zeros(3, 32, dtype=torch.uint8, device=DEV)
+    w4[:, 0] = 2  # 1.0
+    for other in (127, 254 - byte):
+        sw = torch.full((1, 3, 4), other, dtype=torch.uint8, device=DEV)
+        want = _mx_values(q, sq)[:, :1] * 2.0 ** (other - 127)
+        assert torch.equal(ops.gemv_mx_w4(q, sq, w4, sw).double(), want.expand(-1, 3))
+
+
+@gpu
+@pytest.mark.parametrize("act", ["bf16", "fp16", "mx"])
+def test_gemv_4bit_a_scale_of_255_is_nan(act):
+    n, k = 40, 320
+    w4, sw = _weights(n, k, 331)
+    x = _randn((5, k), 332)
+
+    def product(sw, bad_row=None):
+        if act != "mx":
+            return ops.gemv_w4(x.to(torch.bfloat16 if act == "bf16" else torch.float16), w4, sw)
+        q, sq = ops.quantize_mx(x)
+        if bad_row is not None:
+            sq[2, bad_row, 1] = 255
+        return ops.gemv_mx_w4(q, sq, w4, sw)
+
+    want = product(sw)
+    bad = sw.clone()
+    bad[1, 7, 2] = 255
+    got = product(bad)
+    assert bool(got[:, 7].isnan().all())
+    keep = [i for i in range(n) if i != 7]
+    assert torch.equal(got[:, keep], want[:, keep])
+    if act == "mx":
+        got = product(sw, bad_row=3)
+        assert bool(got[3].isnan().all())
+        assert torch.equal(got[[0, 1, 2, 4]], want[[0, 1, 2, 4]])
 
 
 # ---- more rows than one launch has threads for -------------------------------
