@@ -956,6 +956,8 @@ lpx::SampleParam setting(const Setting& v, const char* name, int64_t rows, bool 
     const double d = std::get<double>(v);
     TORCH_CHECK(d >= least && d <= most, "sample: ", name, " must be in [", least, ", ",
                 most, "], got ", d);
+    TORCH_CHECK(!whole || d == std::floor(d), "sample: ", name,
+                " must be a whole number, got ", d);
     return {nullptr, d, lpx::SampleParam::value_};
   }
   const at::Tensor& t = std::get<at::Tensor>(v);

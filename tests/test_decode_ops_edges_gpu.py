@@ -183,6 +183,17 @@ def test_gemv_4bit_refuses_more_weights_than_a_grid_has_threads_for():
         ops.gemv_mx_w4(torch.zeros(1, 64, dtype=torch.uint8),
                        torch.zeros(1, 1, 4, dtype=torch.uint8), w4, sw)
 
+@built
+def test_sample_refuses_a_part_of_a_logit():
+    # top_k counts logits: 2.5 of them was taken as 2, 0.5 as all
+    x, u = torch.zeros(3, 10), torch.zeros(3)
+    for k in (2.5, 0.5, 1e9 + 0.25):
+        with pytest.raises(RuntimeError, match="top_k must be a whole number"):
+            ops.sample(x, u, top_k=k)
+    for k in (0, 2, 2.0, True, 10 ** 12):
+        with pytest.raises(RuntimeError, match="on the ROCm device"):
+            ops.sample(x, u, top_k=k)
+
 
 # ---- sampling: NaN beside infinities ----------------------------------------
 
