@@ -19,11 +19,12 @@
 // workgroup split K step by step, so that together they read neighbouring
 // bytes of a row, and join their sums in LDS in a fixed order.
 //
-// Measured: 100000 x 8192 by one bf16 row 73 us, 5.9 TB/s (reading alone
-// reaches 5.8 to 6.3); 8192 x 8192 by 16 MX rows 8.1 us (10.0 where all of it
-// comes from memory); 28000 x 8192 by 64 MX rows 35 and 44 us, of which the
-// MFMA is busy 12 and the conversions to bf16, LDS and the load path about as
-// long each; 437 tiles on 256 CUs leave a seventh of them idle.
+// Measured: 100000 x 8192 by one bf16 row 74 us, 5.9 TB/s (reading alone
+// reaches 6.4); 8192 x 8192 by 16 MX rows 8.1 us (10.6 where all of it comes
+// from memory); 28000 x 8192 by 64 MX rows 38 and 45 us, of which the MFMA is
+// busy 12 and the conversions to bf16, LDS and the load path about as long
+// each; 437 tiles on 256 CUs leave a seventh of them idle. By 64 bf16 rows 45
+// and 53, fp16 66 and 73.
 
 #include "lpx_common.h"
 #include "kernels.h"

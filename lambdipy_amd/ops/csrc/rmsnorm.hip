@@ -16,8 +16,8 @@
 // step, or two, and a row as many threads as it needs: 16384 x 8192 bf16 with
 // residual to MX 204 us with 256 threads of four steps each, 174 with 1024 of
 // one, 162 where the stores also pass by the caches, 158 (6.0 TB/s) without
-// the code for widths that are no multiple of 8; a copy of that size in torch
-// reaches 4.9.
+// the code for widths that are no multiple of 8; a copy of 2 GiB by a
+// kernel of this form reaches 6.0, torch's 4.9.
 
 #include <algorithm>
 

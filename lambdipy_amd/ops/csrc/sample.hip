@@ -22,10 +22,10 @@
 //
 // f32 rows: a histogram of 256 bins, linear in x below the maximum, tells the
 // bin that holds a border, and only that bin's members are looked at. An exp
-// a logit in 64 bits, 33 instructions, is what that takes; the instructions
+// a logit in 64 bits, some 36 instructions, is what that takes; the instructions
 // bound it. Short rows in one workgroup each; long ones as chunks (maxima,
-// then histograms) and one workgroup a row for the borders: 24 x 50001 25 us,
-// 256 x 131072 96 us.
+// then histograms) and one workgroup a row for the borders: 24 x 50001 26 us,
+// 256 x 131072 94 us, 99 from memory.
 
 #include "lpx_common.h"
 #include "kernels.h"
