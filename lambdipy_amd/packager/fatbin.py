@@ -77,9 +77,10 @@ def source_of(path: str) -> Optional[str]:
 
 def has_fat_binary(path: str) -> bool:
     """Whether a library has HIP code in it, by the names of its sections."""
-    out = subprocess.run(["readelf", "-S", "-W", path], capture_output=True,
-                         text=True, check=True).stdout
-    return ".hip_fatbin" in out.split()
+    r = subprocess.run(["readelf", "-S", "-W", path], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise ValueError(f"{path}: not an ELF file")
+    return ".hip_fatbin" in r.stdout.split()
 
 
 @dataclass

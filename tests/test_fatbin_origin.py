@@ -78,6 +78,14 @@ def test_a_source_newer_than_the_library_is_not_its_source(built, tmp_path):
     assert fatbin.strip_fatbin(str(so))["stripped"] == 1
 
 
+def test_what_is_no_library_is_said_to_be_none(tmp_path):
+    text = tmp_path / "notes.so"
+    text.write_text("no library")
+    with pytest.raises(ValueError, match="not an ELF file"):
+        fatbin.strip_fatbin(str(text))
+    assert text.read_text() == "no library"
+
+
 def test_a_recipe_that_asks_for_it_is_told(monkeypatch):
     # a layer's libraries come out of wheels
     told = []
