@@ -133,9 +133,10 @@ def rmsnorm(x: torch.Tensor, weight: torch.Tensor,
     """Root-mean-square norm over the last axis, of x or of x + residual.
 
     h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight, in f32 (the
-    squares too) from the unrounded h, rounded once. x [..., K] bf16/fp16/f32 (rows may be strided),
-    residual like x, weight [K] of x's type or f32. Returns y, or (y, h) if a
-    residual is given: h, rounded to x's type, is the next layer's residual."""
+    squares too) from the unrounded h, rounded once. x [..., K] bf16/fp16/f32
+    (rows may be strided), residual like x, weight [K] of x's type or f32.
+    Returns y, or (y, h) if a residual is given: h, rounded to x's type, is the
+    next layer's residual."""
     return require_extension().rmsnorm(x, weight, residual, eps)
 
 

@@ -1392,9 +1392,8 @@ SampleParam from_row(SampleParam p, long first) {
   return p;
 }
 
-// Rows to a launch, whose threads are counted in 32 bits: a row takes 1024 in
-// one workgroup, or in chunks no more (they are 4096 logits at least, and more
-// than two a row only where there are few rows).
+// Rows to a launch, whose threads are counted in 32 bits: a row takes 1024, or
+// 256 a chunk, of which there are 2048 more than rows at most.
 constexpr int MOST_ROWS = 1 << 21;
 
 struct Plan {
@@ -1435,12 +1434,12 @@ hipError_t sample(ActType t, const void* logits, long stride, int rows,
   while (vocab > (int64_t(1) << (62 - shift))) --shift;
   char* const work = static_cast<char*>(workspace);
   const SampleArgs a{logits, stride, rows, vocab, p.chunk, p.chunks, shift,
-               temperature, top_k, top_p, min_p, u,
-               reinterpret_cast<ChunkMax*>(work),
-               reinterpret_cast<ChunkBins*>(work + p.bins_at),
-               reinterpret_cast<RowScale*>(work + p.scales_at),
-               temperature.kind != SampleParam::value_ || temperature.value > 0,
-               token};
+                     temperature, top_k, top_p, min_p, u,
+                     reinterpret_cast<ChunkMax*>(work),
+                     reinterpret_cast<ChunkBins*>(work + p.bins_at),
+                     reinterpret_cast<RowScale*>(work + p.scales_at),
+                     temperature.kind != SampleParam::value_ || temperature.value > 0,
+                     token};
   // one launch after the other, in the same workspace
   for (long first = 0; first < rows; first += MOST_ROWS) {
     SampleArgs now = a;
